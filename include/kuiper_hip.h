@@ -156,6 +156,87 @@ int kh_scale_f32(float scale, float* x, int32_t n, void* stream);
 int kh_scale_sum_f32(const float* value, const float* scale, float* out, int32_t pos,
                      int32_t size, int32_t stride, void* stream);
 
+/* ---- many tokens of several sequences -------------------------------------------------------------------
+ * For a program that keeps its own model loop and serves several users (no reference counterpart: its operators know one
+ * token of one sequence).  The tokens of a pass lie one behind the other; offsets [n_seqs + 1] says where each sequence's
+ * begin.  Rows are described by strides, in elements: [token][head][element], the elements of a head side by side.  A query
+ * head h goes with key head h / (head_num / kv_head_num).
+ *
+ * Types: KH_DTYPE_BF16, KH_DTYPE_F32 (sums, softmax and angles in fp32 or more either way).  Pointers are aligned to 16
+ * bytes; head sizes and strides are multiples of 16 bytes; head_size and value_size are at most 256.  Anything else is refused:
+ * KH_ERR_INVALID_ARG, KH_ERR_UNSUPPORTED for the sizes.  No tokens or no sequences: nothing is done.
+ *
+ * A cache of pages: token j of a sequence lies in slot j % page_size of page pages[seq][j / page_size].  Pages may lie in
+ * any order, several sequences may name the same page. */
+typedef struct kh_page_cache {
+  void *k, *v;                                /* [n_pages][page_size][kv_head_num][head_size | value_size] by the strides */
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+  int32_t n_pages, page_size;
+} kh_page_cache;
+
+/* Rotary positions.  Pair i of rot_dim / 2 turns by freq_i = theta^(-2 i / rot_dim) radians a position, after scaling:
+ *   LINEAR  freq / factor
+ *   BANDS   pairs of more than `high` turns within `original` positions stay, those of fewer than `low` are divided by
+ *           factor, in between the two are mixed linearly in the number of turns
+ *   RAMP    the same idea over the pair's number: from floor(pair of `fast` turns) to ceil(pair of `slow` turns); rotated pairs
+ *           are multiplied by `magnitude` (0: 0.1 ln factor + 1)
+ * turns[i] = freq_i / 2 pi as a 64-bit fraction of a turn: position * turns modulo 2^64 is the angle modulo a turn, off by at
+ * most |position| 2^-54 turns (host-only; the caller copies the table to the device). */
+enum { KH_ROPE_SCALE_NONE = 0, KH_ROPE_SCALE_LINEAR = 1, KH_ROPE_SCALE_BANDS = 2, KH_ROPE_SCALE_RAMP = 3 };
+typedef struct kh_rope_scaling {
+  int32_t kind;                                    /* KH_ROPE_SCALE_* */
+  double factor, original, low, high, fast, slow, magnitude;
+} kh_rope_scaling;
+int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scaling* scaling /* may be NULL */, uint64_t* h_turns,
+                  float* h_magnitude);
+
+/* The first rot_dim elements of every head are rotated by their token's position (any int32), the others pass; mode as in
+ * kh_rope_f32.  q_out / k_out may be q / k (with the same strides); they may not overlap them otherwise. */
+typedef struct kh_rope_rows {
+  int32_t dtype, mode, n_tokens, head_num, kv_head_num, head_size, rot_dim;
+  float magnitude;
+  const uint64_t* turns;      /* [rot_dim / 2], from kh_rope_turns */
+  const int32_t* positions;   /* [n_tokens] */
+  const void *q, *k;
+  int64_t q_token, q_head, k_token, k_head;
+  void *q_out, *k_out;        /* k_out: kh_rope_tokens only */
+  int64_t qo_token, qo_head, ko_token, ko_head;
+} kh_rope_rows;
+int kh_rope_tokens(const kh_rope_rows* r, void* stream);
+/* The same with the rotated keys, and the values as they are, written into a cache of pages: token t to slot
+ * slots[t] % page_size of page slots[t] / page_size.  A negative slot, or one behind the cache, stores nothing (the query is
+ * rotated all the same); no two tokens may have the same one. */
+int kh_rope_store(const kh_rope_rows* r, const void* v, int64_t v_token, int64_t v_head, int32_t value_size,
+                  const kh_page_cache* cache, const int32_t* slots, void* stream);
+
+/* Causal attention.  Query i of a sequence with n tokens here and `length` keys stands at place p = length - n + i and sees
+ * the keys j with p - window < j <= p (window <= 0: all up to p); out = sum_j softmax_j(scale q . k_j) v_j, scale > 0.  A query
+ * that sees no key gets zeros.  Rows behind the last sequence are left as they were.  Keys that a query does not see do not
+ * reach it, whatever they hold. */
+typedef struct kh_attn_rows {
+  int32_t dtype, n_tokens, n_seqs, head_num, kv_head_num, head_size, value_size, window;
+  float scale;
+  const int32_t* offsets;     /* [n_seqs + 1], ascending, at most n_tokens */
+  const void* q;              /* [n_tokens][head_num][head_size] */
+  int64_t q_token, q_head;
+  void* out;                  /* [n_tokens][head_num][value_size]; may not overlap q */
+  int64_t o_token, o_head;
+} kh_attn_rows;
+/* Whole prompts: the keys and values of a sequence are the rows of its own tokens. */
+int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                   int64_t v_head, void* stream);
+/* New tokens of each sequence (any number, none too) over the lengths[seq] keys that the cache holds of it, its new ones among
+ * them.  pages: rows of page numbers, table_width of them a sequence, table_stride apart.  A page outside the cache or a
+ * length behind the table makes rows that would need it NaN, and maybe others of that sequence; pages that no query of the
+ * pass sees (behind the length, before the window) are not looked at.  max_new: the most new tokens that the caller
+ * expects of any sequence (0: not known); it chooses between kernels and changes no result but by the order of sums.
+ * workspace = kh_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, contents of no account before and after; two calls
+ * that may run at the same time need one each. */
+int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens);
+int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* cache, const int32_t* pages, int64_t table_stride,
+                  int32_t table_width, const int32_t* lengths, int32_t max_new, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
 /* ============================ model level ==============================================
  * Replaces model::LLama2Model / Qwen2Model for the decode path: .bin image -> HBM arena,
  * per-token forward, greedy generate loop captured in a hipGraph. */

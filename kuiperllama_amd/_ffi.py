@@ -19,6 +19,7 @@ EXPORTS = [
     "kh_rmsnorm_f32", "kh_rope_f32", "kh_sincos_cache_f32", "kh_mha_f32", "kh_mha_decode_f32", "kh_mha_prefill_f32",
     "kh_mha_decode_workspace_bytes", "kh_argmax_f32",
     "kh_argmax_f32_host", "kh_softmax_f32", "kh_scale_f32", "kh_scale_sum_f32",
+    "kh_rope_turns", "kh_rope_tokens", "kh_rope_store", "kh_attn_packed", "kh_attn_paged", "kh_attn_paged_workspace_bytes",
     "kh_model_create_from_file", "kh_model_create_from_host_image",
     "kh_model_create_from_device_weights", "kh_model_destroy", "kh_model_get_config",
     "kh_model_stream", "kh_model_get_load_ms", "kh_model_predict", "kh_model_get_logits", "kh_model_get_kv", "kh_model_kv_bytes", "kh_model_read_kv", "kh_model_write_kv",
@@ -75,6 +76,28 @@ class Config(C.Structure):
                                       ("ring_selftest", C.c_int32), ("attn_merge_selftest", C.c_int32)]
 
 
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32)] + [(n, C.c_double) for n in ("factor", "original", "low", "high", "fast", "slow", "magnitude")]
+
+
+class PageCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in ("k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head")] + \
+               [("n_pages", C.c_int32), ("page_size", C.c_int32)]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "mode", "n_tokens", "head_num", "kv_head_num", "head_size", "rot_dim")] + \
+               [("magnitude", C.c_float), ("turns", C.c_void_p), ("positions", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head")] + [("q_out", C.c_void_p), ("k_out", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("qo_token", "qo_head", "ko_token", "ko_head")]
+
+
+class AttnRows(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "n_tokens", "n_seqs", "head_num", "kv_head_num", "head_size", "value_size", "window")] + \
+               [("scale", C.c_float), ("offsets", C.c_void_p), ("q", C.c_void_p), ("q_token", C.c_int64), ("q_head", C.c_int64),
+                ("out", C.c_void_p), ("o_token", C.c_int64), ("o_head", C.c_int64)]
+
+
 _lib: Optional[C.CDLL] = None
 _vp, _i32, _i64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
@@ -118,6 +141,13 @@ def lib() -> C.CDLL:
     L.kh_softmax_f32.argtypes = [_vp, _i32, _vp]
     L.kh_scale_f32.argtypes = [_f32, _vp, _i32, _vp]
     L.kh_scale_sum_f32.argtypes = [_vp, _vp, _vp, _i32, _i32, _i32, _vp]
+    L.kh_rope_turns.argtypes = [_i32, C.c_double, C.POINTER(RopeScaling), C.POINTER(C.c_uint64), C.POINTER(_f32)]
+    L.kh_rope_tokens.argtypes = [C.POINTER(RopeRows), _vp]
+    L.kh_rope_store.argtypes = [C.POINTER(RopeRows), _vp, _i64, _i64, _i32, C.POINTER(PageCache), _vp, _vp]
+    L.kh_attn_packed.argtypes = [C.POINTER(AttnRows), _vp, _i64, _i64, _vp, _i64, _i64, _vp]
+    L.kh_attn_paged_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32]
+    L.kh_attn_paged_workspace_bytes.restype = _i64
+    L.kh_attn_paged.argtypes = [C.POINTER(AttnRows), C.POINTER(PageCache), _vp, _i64, _i32, _vp, _i32, _vp, _i64, _vp]
     L.kh_model_create_from_file.argtypes = [C.c_char_p, C.POINTER(ModelOpts), C.POINTER(_vp)]
     L.kh_model_create_from_host_image.argtypes = [_vp, C.c_size_t, C.POINTER(ModelOpts),
                                                   C.POINTER(_vp)]

@@ -1,0 +1,133 @@
+// kh_seqattn.hip — attention of many sequences' tokens: checks and launches (kernels in kh_seqattn.h).
+#include "kh_seqattn.h"
+
+#include <limits.h>
+
+namespace khm {
+namespace {
+
+bool whole(int64_t n, int esize) { return n % (16 / esize) == 0; }
+
+// Common checks; *todo = 0: nothing to do.
+int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
+  *todo = 0;
+  if (!r || (r->dtype != KH_DTYPE_BF16 && r->dtype != KH_DTYPE_F32) || r->n_tokens < 0 || r->n_seqs < 0 || r->head_num <= 0 ||
+      r->kv_head_num <= 0 || r->head_num % r->kv_head_num || r->head_size <= 0 || r->value_size <= 0 || !(r->scale > 0.f) ||
+      !(r->scale < INFINITY))
+    return KH_ERR_INVALID_ARG;
+  const int e = *esize = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
+  if (!whole(r->head_size, e) || !whole(r->value_size, e) || r->head_size > 256 || r->value_size > 256) return KH_ERR_UNSUPPORTED;
+  // rows of a sequence are counted in 32 bits, and so are the workgroups
+  if ((int64_t)r->n_tokens * r->head_num > INT_MAX / 2 || r->n_seqs > INT_MAX / 2 / r->kv_head_num) return KH_ERR_UNSUPPORTED;
+  if (r->n_tokens == 0 || r->n_seqs == 0) return KH_OK;
+  if (!r->offsets || !r->q || !r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !whole(r->q_token, e) || !whole(r->q_head, e) ||
+      !whole(r->o_token, e) || !whole(r->o_head, e))
+    return KH_ERR_INVALID_ARG;
+  *todo = 1;
+  return KH_OK;
+}
+
+SeqArgs args_of(const kh_attn_rows* r, int e) {
+  SeqArgs a{};
+  a.q = (const char*)r->q;
+  a.out = (char*)r->out;
+  a.q_token = r->q_token * e;
+  a.q_head = r->q_head * e;
+  a.o_token = r->o_token * e;
+  a.o_head = r->o_head * e;
+  a.offsets = r->offsets;
+  a.n_tokens = r->n_tokens;
+  a.n_seqs = r->n_seqs;
+  a.heads = r->head_num;
+  a.kv_heads = r->kv_head_num;
+  a.group = r->head_num / r->kv_head_num;
+  a.kchunks = r->head_size * e / 16;
+  a.vchunks = r->value_size * e / 16;
+  a.window = r->window;
+  a.c = r->scale * 1.4426950408889634f;
+  return a;
+}
+
+template <class K>
+int launch(K kern, unsigned grid, int threads, int lds, const SeqArgs& a, hipStream_t s) {
+  if (lds > 64 * 1024) KH_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(threads), lds, s, a);
+  return kh_launch_status();
+}
+
+template <class T, int DP, bool PAGED>
+int tiles(const SeqArgs& a, hipStream_t s) {
+  typedef SeqTiles<T, DP> S;
+  const int64_t slots = (int64_t)a.n_tokens * a.group / S::BM + a.n_seqs;
+  return launch(k_seq_tiles<T, DP, PAGED>, (unsigned)(slots * a.kv_heads), 64 * S::W, S::LDS, a, s);
+}
+
+template <bool PAGED>
+int go(const SeqArgs& a, int e, hipStream_t s) {
+  const int most = (a.kchunks > a.vchunks ? a.kchunks : a.vchunks) * 16 / e;
+  if (e == 2) return most <= 64 ? tiles<bf16, 64, PAGED>(a, s) : (most <= 128 ? tiles<bf16, 128, PAGED>(a, s) : tiles<bf16, 256, PAGED>(a, s));
+  return most <= 64 ? tiles<float, 64, PAGED>(a, s) : (most <= 128 ? tiles<float, 128, PAGED>(a, s) : tiles<float, 256, PAGED>(a, s));
+}
+}  // namespace
+}  // namespace khm
+
+extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, void* stream) {
+  int e, todo;
+  const int rc = khm::check_rows(r, &e, &todo);
+  if (rc != KH_OK || !todo) return rc;
+  if (!k || !v || !kh_aligned16(k) || !kh_aligned16(v) || !khm::whole(k_token, e) || !khm::whole(k_head, e) || !khm::whole(v_token, e) ||
+      !khm::whole(v_head, e))
+    return KH_ERR_INVALID_ARG;
+  khm::SeqArgs a = khm::args_of(r, e);
+  a.kv.k = (const char*)k;
+  a.kv.v = (const char*)v;
+  a.kv.k_slot = k_token * e;
+  a.kv.k_head = k_head * e;
+  a.kv.v_slot = v_token * e;
+  a.kv.v_head = v_head * e;
+  return khm::go<false>(a, e, (hipStream_t)stream);
+}
+
+extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
+  if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
+  return 16;
+}
+
+extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
+                             int32_t table_width, const int32_t* lengths, int32_t max_new, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  int e, todo;
+  const int rc = khm::check_rows(r, &e, &todo);
+  if (rc != KH_OK) return rc;
+  if (!c || c->n_pages <= 0 || c->page_size <= 0 || c->page_size > 1 << 20 || table_width <= 0 || table_stride < 0 || max_new < 0)
+    return KH_ERR_INVALID_ARG;
+  if (!todo) return KH_OK;
+  if (!c->k || !c->v || !pages || !lengths || !kh_aligned16(c->k) || !kh_aligned16(c->v) || !khm::whole(c->k_page, e) ||
+      !khm::whole(c->k_slot, e) || !khm::whole(c->k_head, e) || !khm::whole(c->v_page, e) || !khm::whole(c->v_slot, e) ||
+      !khm::whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
+      workspace_bytes < kh_attn_paged_workspace_bytes(r->head_num, r->kv_head_num, r->value_size, r->n_tokens))
+    return KH_ERR_INVALID_ARG;
+  khm::SeqArgs a = khm::args_of(r, e);
+  a.kv.k = (const char*)c->k;
+  a.kv.v = (const char*)c->v;
+  a.kv.k_page = c->k_page * e;
+  a.kv.k_slot = c->k_slot * e;
+  a.kv.k_head = c->k_head * e;
+  a.kv.v_page = c->v_page * e;
+  a.kv.v_slot = c->v_slot * e;
+  a.kv.v_head = c->v_head * e;
+  a.kv.pages = pages;
+  a.kv.table_stride = table_stride;
+  a.kv.most = (int64_t)table_width * c->page_size < INT_MAX / 2 ? table_width * c->page_size : INT_MAX / 2;
+  a.kv.n_pages = c->n_pages;
+  a.kv.page_size = c->page_size;
+  // for d = page_size >= 2, 2^(b-1) < d <= 2^b: floor(2^(31+b) / d) + 1 is too large by at most 1, so its product with n < 2^31 by
+  // less than 2^(31+b) / d, and the quotient is exact
+  int bits = 0;
+  while ((1 << bits) < c->page_size) ++bits;
+  a.kv.magic = c->page_size == 1 ? 0 : (uint32_t)((1ull << (31 + bits)) / (uint64_t)c->page_size + 1);
+  a.kv.shift = bits - 1;
+  a.kv.lengths = lengths;
+  return khm::go<true>(a, e, (hipStream_t)stream);
+}

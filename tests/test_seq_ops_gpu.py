@@ -1,0 +1,494 @@
+"""Operators over many tokens of several sequences against their formulas in 64 bits: rope_tokens, rope_store, attn_packed,
+attn_paged (kuiperllama_amd.ops).
+
+Tolerances, from the roundings alone (u = 2^-24, h = half a step of the storage type: 2^-8 for bf16, u for fp32):
+
+  rotation    cosine and sine are off by at most 4 u (angle: two conversions and a product, 3 u of at most 0.79; polynomial: 1.5 u; what
+              it leaves out: 0.1 u), their products with the factor, with the elements and the sum of two take 4 u more, and the
+              result is rounded once: 8 u f (|a| + |b|) + h |x'|
+  attention   a score of n products is off by at most (n + 1) u sum |q k|, its exponent by that times c = scale log2 e and by 3 u
+              (|c s| + |c m|) for the fma and its base, the exponential by 2 u more; weights for bf16 are rounded (h); sums of N
+              terms take N u.  A weight's relative error e enters the output twice, over the weights and over their sum:
+              (2 e + 2 N u + h [bf16]) sum w |v| + 2 h |out|
+"""
+import math
+
+import pytest
+import torch
+
+from test_seq_ops import SCALINGS, frequencies
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rnd(gen, dtype, *shape, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=gen) * scale).to(dtype)
+
+
+def generator(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+# ---- the formulas ----------------------------------------------------------------------------------------------------
+def rotated(x, positions, rot, theta, scaling, half):
+    """-> (x', bound of the error of rounding) in 64 bits."""
+    f, factor = frequencies(rot, theta, scaling)
+    angle = positions.double()[:, None] * torch.tensor(f, dtype=torch.float64, device=x.device)
+    cos, sin = (angle.cos() * factor)[:, None, :], (angle.sin() * factor)[:, None, :]
+    y, bound = x.double().clone(), torch.zeros_like(x, dtype=torch.float64)
+    i = torch.arange(rot // 2, device=x.device)
+    a, b = (i, i + rot // 2) if half else (2 * i, 2 * i + 1)
+    u, v = x.double()[..., a], x.double()[..., b]
+    y[..., a], y[..., b] = u * cos - v * sin, u * sin + v * cos
+    # and the table: |position| 2^-54 turns, and this side's own angle, |angle| 2^-53
+    bound[..., a] = bound[..., b] = (8 * U + (positions.double().abs() * 2 ** -50)[:, None, None]) * factor * (u.abs() + v.abs())
+    return y, bound + half_step(x.dtype) * y.abs() * (1 if rot else 0)
+
+
+def attended(q, k, v, window, scale):
+    """One sequence: n queries at the last n of the keys; -> (out, bound) in 64 bits."""
+    n, heads, _ = q.shape
+    L, kv = k.shape[:2]
+    out = torch.zeros(n, heads, v.shape[2], dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    place = torch.arange(L - n, L, device=q.device)[:, None]
+    j = torch.arange(L, device=q.device)[None, :]
+    seen = (j <= place) & ((j > place - window) if window > 0 else True)
+    any_seen = seen.any(1)
+    c = scale * math.log2(math.e)
+    h = half_step(q.dtype)
+    for head in range(heads):
+        kd, vd, qd = k[:, head * kv // heads].double(), v[:, head * kv // heads].double(), q[:, head].double()
+        s = (qd @ kd.t()) * scale
+        size = (qd.abs() @ kd.abs().t()) * scale
+        s = s.masked_fill(~seen, -math.inf)
+        m = s.amax(1, keepdim=True).masked_fill(~any_seen[:, None], 0.0)
+        p = torch.exp(s - m)
+        w = p / p.sum(1, keepdim=True).clamp_min(1e-300)
+        out[:, head] = w @ vd
+        top = size.masked_fill(~seen, 0.0).amax(1, keepdim=True)  # |s|, |m| are below it too
+        e = (q.shape[2] + 1 + 6) * U * top + 4 * U
+        bound[:, head] = (2 * e + 2 * L * U + (h if q.dtype == BF16 else 0.0)) * (w @ vd.abs()) + 2 * h * out[:, head].abs()
+    return out, bound
+
+
+def close(got, want, bound, what=""):
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound + 1e-30)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / (bound + 1e-30)).nan_to_num(1e9).max()):.3g} of the bound"
+
+
+# ---- rotations -------------------------------------------------------------------------------------------------------
+ROTATIONS = [  # tokens, heads, kv_heads, size, rot, theta, farthest position
+    (1, 32, 8, 64, 64, 5e5, 131072), (33, 14, 2, 64, 64, 1e6, 4096), (5, 6, 6, 48, 48, 1e4, 256), (70, 4, 1, 128, 64, 1e4, 1 << 20),
+    (9, 32, 32, 128, 128, 1e4, 4096), (3, 8, 4, 80, 40, 1e4, 8192), (4, 2, 1, 80, 20, 1e4, 8192), (17, 3, 1, 256, 254, 1e4, 4096), (2, 5, 5, 8, 2, 10.0, 99),
+    (300, 12, 2, 96, 0, 1e4, 10)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("half", [True, False], ids=["half", "pairs"])
+@pytest.mark.parametrize("shape", ROTATIONS, ids=str)
+def test_rotation(gpu, dtype, half, shape):
+    from kuiperllama_amd import ops
+    T, H, KH, D, rot, theta, far = shape
+    gen = generator(T * D + rot)
+    rows = rnd(gen, dtype, T, (H + 2 * KH) * D + 16)  # rows that q, k and v are slices of
+    q, k, v = (rows[:, a * D:(a + n) * D].view(T, n, D) for a, n in ((0, H), (H, KH), (H + KH, KH)))
+    scaling = SCALINGS[(T + D) % len(SCALINGS)]
+    pos = torch.randint(0, far, (T,), device=gpu, generator=gen, dtype=torch.int32)
+    table = ops.rope_table(rot, theta, gpu, scaling)
+    mode = ops.ROPE_HALF if half else ops.ROPE_INTERLEAVED
+    wants = [rotated(x, pos, rot, theta, scaling, half) for x in (q, k)]
+    before = rows.clone()
+    q2, k2 = torch.full((T, H, D), 7.0, dtype=dtype, device=gpu), torch.full((T, KH, D), 7.0, dtype=dtype, device=gpu)
+    assert ops.rope_tokens(q, k, pos, table, mode, q_out=q2, k_out=k2)[0] is q2
+    assert torch.equal(rows, before)
+    close(q2, *wants[0], "q")
+    close(k2, *wants[1], "k")
+    assert torch.equal(q2[..., rot:], q[..., rot:])
+    # into a cache: every place that no token has stays
+    page = 16 if T % 2 else 5
+    pages = T // page + 3
+    kc, vc = (torch.full((pages, KH, page, D), 5.0, dtype=dtype, device=gpu).transpose(1, 2) for _ in range(2))  # heads outside the slots
+    slots = torch.randperm(pages * page, device=gpu, generator=gen)[:T].to(torch.int32)
+    if T > 2:
+        slots[1], slots[2] = -1, pages * page  # nowhere
+    kwant, vwant = kc.clone(), vc.clone()
+    q3 = torch.full_like(q2, 7.0)
+    ops.rope_store(q, k, v, pos, table, mode, kc, vc, slots, q_out=q3)
+    for t in range(T):
+        s = int(slots[t])
+        if 0 <= s < pages * page:
+            kwant[s // page, s % page], vwant[s // page, s % page] = k2[t], v[t]
+    assert torch.equal(q3, q2) and torch.equal(kc, kwant) and torch.equal(vc, vwant)
+    # in place
+    ops.rope_tokens(q, k, pos, table, mode)
+    assert torch.equal(q, q2) and torch.equal(k, k2)
+    assert torch.equal(rows[:, (H + KH) * D:], before[:, (H + KH) * D:])
+
+
+def test_rotation_far_and_behind(gpu):
+    """Positions of either sign up to the ends of int32, where fp32 angles hold nothing."""
+    from kuiperllama_amd import ops
+    pos = torch.tensor([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 10 ** 9, 1 << 24, -(1 << 24) - 1], dtype=torch.int32, device=gpu)
+    gen = generator(5)
+    q, k = rnd(gen, F32, 8, 3, 64), rnd(gen, F32, 8, 1, 64)
+    q2, k2 = torch.empty_like(q), torch.empty_like(k)
+    ops.rope_tokens(q, k, pos, ops.rope_table(64, 1e4, gpu), ops.ROPE_HALF, q2, k2)
+    close(q2, *rotated(q, pos, 64, 1e4, None, True))
+    close(k2, *rotated(k, pos, 64, 1e4, None, True))
+    assert torch.equal(q2[0], q[0])  # position 0
+
+
+# ---- packed prompts --------------------------------------------------------------------------------------------------
+def offsets_of(lens, device):
+    return torch.tensor([0] + list(torch.tensor(lens, dtype=torch.int64).cumsum(0)), dtype=torch.int32, device=device)
+
+
+PACKED = [  # heads, kv_heads, key size, value size, lengths, window
+    (14, 2, 64, 64, [7, 33, 1], 0), (32, 8, 64, 64, [300, 0, 128, 129, 1, 64], 0), (4, 4, 128, 128, [513], 0), (6, 6, 48, 48, [31, 32, 33, 65], 0),
+    (12, 1, 128, 128, [100, 11], 0), (8, 2, 64, 64, [500, 20], 100), (8, 8, 64, 64, [200], 1), (3, 1, 80, 40, [150, 3], 64), (5, 5, 16, 256, [130], 0),
+    (4, 2, 256, 256, [140, 70], 37), (7, 1, 192, 128, [90], 0), (2, 1, 8, 8, [40, 1, 1], 0), (1, 1, 64, 64, [1030], 129), (64, 1, 64, 64, [9, 2], 0)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", PACKED, ids=str)
+def test_packed(gpu, dtype, case):
+    from kuiperllama_amd import ops
+    H, KH, D, DV, lens, window = case
+    gen = generator(sum(lens) + D)
+    T, behind = sum(lens), 3  # rows of a padded batch
+    rows = rnd(gen, dtype, T + behind, H * D + KH * (D + DV) + 8)
+    q = rows[:, :H * D].view(T + behind, H, D)
+    k = rows[:, H * D:(H + KH) * D].view(T + behind, KH, D)
+    v = rows[:, (H + KH) * D:(H + KH) * D + KH * DV].view(T + behind, KH, DV)
+    out = torch.full((T + behind, H, DV), 9.0, dtype=dtype, device=gpu)
+    assert ops.attn_packed(q, k, v, offsets_of(lens, gpu), out, window=window) is out
+    first = 0
+    for n in lens:
+        s = slice(first, first + n)
+        if n:
+            close(out[s], *attended(q[s], k[s], v[s], window, D ** -0.5), f"length {n}")
+        first += n
+    assert (out[T:] == 9.0).all()
+    if H == KH == 4:  # a scale of one's own
+        ops.attn_packed(q, k, v, offsets_of(lens, gpu), out, scale=0.5)
+        close(out[:T], *attended(q[:T], k[:T], v[:T], 0, 0.5), "scale")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_what_a_query_does_not_see_does_not_reach_it(gpu, dtype):
+    """Infinities and NaN in keys and values of later tokens, and of tokens before the window."""
+    from kuiperllama_amd import ops
+    gen = generator(3)
+    H, KH, D, n, window = 4, 2, 64, 150, 20
+    q, k, v = rnd(gen, dtype, n, H, D), rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, D)
+    want, bound = attended(q, k, v, window, D ** -0.5)
+    for t, value in ((40, math.inf), (41, math.nan), (75, -math.inf)):
+        v[t, :, t % 7::5] = value
+    k[100] = math.nan
+    k[149, 1, 3] = math.inf
+    out = torch.empty(n, H, D, dtype=dtype, device=gpu)
+    ops.attn_packed(q, k, v, offsets_of([n], gpu), out, window=window)
+    rows = torch.arange(n, device=gpu)
+    hit = torch.zeros(n, H, D, dtype=torch.bool, device=gpu)
+    for t in (40, 41, 75):
+        hit[(rows >= t) & (rows < t + window), :, t % 7::5] = True
+    hit[(rows >= 100) & (rows < 100 + window)] = True
+    hit[149, 2:] = True
+    close(out[~hit], want[~hit], bound[~hit])
+    assert not torch.isfinite(out[rows < 100][hit[rows < 100]]).any()
+    at40 = out[40, :, 40 % 7::5]
+    assert (at40 == math.inf).all()
+    assert torch.isnan(out[100:100 + window]).all()
+
+
+def test_scores_of_any_size(gpu):
+    """Rows whose scores differ by thousands, and whose maximum comes late."""
+    from kuiperllama_amd import ops
+    gen = generator(8)
+    n, H, D = 200, 2, 64
+    q = rnd(gen, F32, n, H, D)
+    k, v = rnd(gen, F32, n, H, D) * torch.linspace(0.1, 60, n, device=gpu)[:, None, None], rnd(gen, F32, n, H, D)
+    out = torch.empty_like(q)
+    ops.attn_packed(q, k, v, offsets_of([n], gpu), out, scale=1.0)
+    close(out, *attended(q, k, v, 0, 1.0))
+
+
+# ---- a cache of pages ------------------------------------------------------------------------------------------------
+def paged(gen, dtype, KH, D, DV, lens, page, spare=3, heads_first=False):
+    """A cache whose unused places hold NaN, its table with pages that are none behind each sequence's last, and the keys and values
+    of each sequence."""
+    held = [-(-n // page) for n in lens]
+    total = sum(held) + spare
+
+    def make(size):
+        if heads_first:
+            return torch.full((total, KH, page, size), math.nan, dtype=dtype, device="cuda").transpose(1, 2)
+        return torch.full((total, page, KH, size), math.nan, dtype=dtype, device="cuda")
+
+    kc, vc = make(D), make(DV)
+    order = torch.randperm(total, generator=gen, device="cuda")[:sum(held)]
+    table = torch.full((len(lens), max(max(held), 1) + 2), -1, dtype=torch.int32, device="cuda")
+    at, ks, vs = 0, [], []
+    for b, n in enumerate(lens):
+        mine = order[at:at + held[b]]
+        at += held[b]
+        table[b, :held[b]] = mine.to(torch.int32)
+        k, v = rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, DV)
+        j = torch.arange(n, device="cuda")
+        kc[mine[j // page], j % page], vc[mine[j // page], j % page] = k, v
+        ks.append(k)
+        vs.append(v)
+    return kc, vc, table, ks, vs
+
+
+PAGED = [  # heads, kv_heads, key size, value size, new tokens, lengths, page, window
+    (32, 8, 64, 64, [1] * 5, [1, 16, 17, 700, 64], 16, 0), (32, 8, 128, 128, [1, 1, 1], [4000, 3, 129], 64, 0), (14, 2, 64, 64, [1, 2, 0, 5], [40, 2, 9, 300], 24, 0),
+    (8, 2, 64, 64, [200, 1, 33], [900, 1000, 33], 48, 0), (4, 4, 128, 128, [64], [1000], 128, 0), (12, 1, 64, 64, [1, 3], [333, 77], 1, 0),
+    (32, 4, 64, 64, [1, 70, 1], [500, 300, 20], 16, 100), (6, 6, 48, 48, [1, 1], [256, 31], 100, 31), (8, 8, 256, 256, [1, 40], [90, 100], 16, 0),
+    (3, 1, 80, 40, [2, 9], [50, 9], 7, 5), (2, 2, 64, 64, [3, 1, 4], [1, 0, 4], 16, 0), (64, 1, 128, 128, [1], [600], 32, 0), (1, 1, 16, 16, [1], [5000], 256, 0),
+    (32, 8, 64, 64, [8, 4], [515, 1027], 64, 0), (16, 1, 192, 128, [1, 2], [300, 100], 64, 0), (32, 8, 64, 64, [1] * 70, list(range(1, 141, 2)), 16, 0)]
+
+
+def check_paged(q, out, lens, new, ks, vs, window, what=""):
+    first, D = 0, q.shape[2]
+    for b, (n, length) in enumerate(zip(new, lens)):
+        if n > length:  # queries before the first key see nothing
+            assert (out[first:first + n - length] == 0).all(), what
+            m = length
+        else:
+            m = n
+        if m:
+            s = slice(first + n - m, first + n)
+            close(out[s], *attended(q[s], ks[b], vs[b], window, D ** -0.5), f"{what} sequence {b}: {n} of {length}")
+        first += n
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", PAGED, ids=lambda c: str(c)[:60])
+def test_paged(gpu, dtype, case):
+    from kuiperllama_amd import ops
+    H, KH, D, DV, new, lens, page, window = case
+    gen = generator(sum(lens) + D + page)
+    kc, vc, table, ks, vs = paged(gen, dtype, KH, D, DV, lens, page, heads_first=len(lens) % 2 == 0)
+    T = sum(new)
+    q = rnd(gen, dtype, T + 2, H, D, scale=1.5)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ws = ops.attn_paged_workspace(H, KH, DV, T + 2, gpu)
+    for max_new in (None, max(new), 1):  # the last may be wrong: it may change no result but by the order of sums
+        out = torch.full((T + 2, H, DV), 9.0, dtype=dtype, device=gpu)
+        ws.fill_(0xff)
+        assert ops.attn_paged(q, kc, vc, table, lengths, offsets_of(new, gpu), out, ws, window=window, max_new=max_new) is out
+        check_paged(q, out, lens, new, ks, vs, window, f"max_new {max_new}")
+        assert (out[T:] == 9.0).all()
+    if window:  # pages before the window belong to someone else by now
+        for b, (n, length) in enumerate(zip(new, lens)):
+            gone = max(0, length - n - window + 1) // page
+            table[b, :gone] = torch.tensor([-7, 1 << 30], device=gpu, dtype=torch.int32).repeat(gone)[:gone]
+        again = torch.full_like(out, 9.0)
+        ops.attn_paged(q, kc, vc, table, lengths, offsets_of(new, gpu), again, ws, window=window, max_new=max_new)
+        assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 1]], ids=str)
+def test_pages_and_lengths_that_are_none(gpu, new):
+    """A page number outside the cache and a length behind the table: NaN for the sequence that needs it, the others as ever."""
+    from kuiperllama_amd import ops
+    gen = generator(21)
+    H, KH, D, page, lens = 8, 2, 64, 16, [200, 150, 90]
+    kc, vc, table, ks, vs = paged(gen, BF16, KH, D, D, lens, page)
+    q = rnd(gen, BF16, sum(new), H, D)
+    ws = ops.attn_paged_workspace(H, KH, D, sum(new), gpu)
+    off = offsets_of(new, gpu)
+    good = torch.empty(sum(new), H, D, dtype=BF16, device=gpu)
+    ops.attn_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=gpu), off, good, ws)
+    check_paged(q, good, lens, new, ks, vs, 0)
+    for number in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
+        broken = table.clone()
+        broken[1, 3] = number
+        out = torch.zeros_like(good)
+        ops.attn_paged(q, kc, vc, broken, torch.tensor(lens, dtype=torch.int32, device=gpu), off, out, ws)
+        b = slice(new[0], new[0] + 1)
+        assert torch.isnan(out[b]).all() and torch.equal(out[:new[0]], good[:new[0]]) and torch.equal(out[new[0] + 1:], good[new[0] + 1:])
+    long = torch.tensor([lens[0], lens[1], table.shape[1] * page + 1000], dtype=torch.int32, device=gpu)
+    out = torch.zeros_like(good)
+    ops.attn_paged(q, kc, vc, table, long, off, out, ws)
+    assert torch.isnan(out[-1]).all() and torch.equal(out[:-1], good[:-1])
+
+
+def test_sequences_that_share_pages(gpu):
+    """Two sequences with the same beginning."""
+    from kuiperllama_amd import ops
+    gen = generator(4)
+    kc, vc, table, ks, vs = paged(gen, F32, 2, 64, 64, [64, 40, 1], 16)
+    table[1, :2] = table[0, :2]
+    ks[1], vs[1] = torch.cat([ks[0][:32], ks[1][32:]]), torch.cat([vs[0][:32], vs[1][32:]])
+    q = rnd(gen, F32, 12, 4, 64)
+    out, ws = torch.empty(12, 4, 64, device=gpu), ops.attn_paged_workspace(4, 2, 64, 12, gpu)
+    ops.attn_paged(q, kc, vc, table, torch.tensor([64, 40, 1], dtype=torch.int32, device=gpu), offsets_of([1, 10, 1], gpu), out, ws)
+    check_paged(q, out, [64, 40, 1], [1, 10, 1], ks, vs, 0)
+
+
+# ---- together --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_a_layer_s_attention_in_portions(gpu, dtype):
+    """Three prompts, whole, against the same tokens in portions over a cache, then single tokens in a captured graph whose lengths,
+    slots and positions move on the device."""
+    from kuiperllama_amd import ops
+    gen = generator(77)
+    H, KH, D, page, lens, steps = 8, 2, 64, 16, [150, 37, 90], 6
+    whole = [n + steps for n in lens]
+    raw = [(rnd(gen, dtype, n, H, D, scale=2.0), rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, D)) for n in whole]
+    table = ops.rope_table(D, 5e5, gpu, SCALINGS[3])
+    mode = ops.ROPE_HALF
+    # whole prompts
+    q, k, v = (torch.cat([r[i] for r in raw]) for i in range(3))
+    pos = torch.cat([torch.arange(n, device=gpu, dtype=torch.int32) for n in whole])
+    qr, kr = torch.empty_like(q), torch.empty_like(k)
+    ops.rope_tokens(q, k, pos, table, mode, qr, kr)
+    want = torch.empty_like(q)
+    ops.attn_packed(qr, kr, v, offsets_of(whole, gpu), want)
+    first = [0, whole[0], whole[0] + whole[1]]
+    bounds = [attended(qr[f:f + n], kr[f:f + n], v[f:f + n], 0, D ** -0.5) for f, n in zip(first, whole)]
+    for b in range(3):
+        close(want[first[b]:first[b] + whole[b]], *bounds[b], "whole")
+    # portions
+    held = [-(-n // page) for n in whole]
+    kc = torch.full((sum(held) + 1, page, KH, D), math.nan, dtype=dtype, device=gpu)
+    vc = torch.full_like(kc, math.nan)
+    pages = torch.zeros(3, max(held), dtype=torch.int32, device=gpu)
+    order = torch.randperm(sum(held), device=gpu, generator=gen).to(torch.int32)
+    for b, part in enumerate(order.split(held)):
+        pages[b, :held[b]] = part
+    done = [0, 0, 0]
+    for portion in ([64, 37, 1], [60, 0, 89], [26, 0, 0]):
+        x = [torch.cat([raw[b][i][done[b]:done[b] + portion[b]] for b in range(3)]) for i in range(3)]
+        p = torch.cat([torch.arange(done[b], done[b] + portion[b], device=gpu, dtype=torch.int32) for b in range(3)])
+        seq = torch.cat([torch.full((portion[b],), b, device=gpu) for b in range(3)])
+        slots = pages[seq, p.long() // page] * page + p % page
+        ops.rope_store(x[0], x[1], x[2], p, table, mode, kc, vc, slots)
+        done = [a + n for a, n in zip(done, portion)]
+        out, ws = torch.empty_like(x[0]), ops.attn_paged_workspace(H, KH, D, sum(portion), gpu)
+        ops.attn_paged(x[0], kc, vc, pages, torch.tensor(done, dtype=torch.int32, device=gpu), offsets_of(portion, gpu), out, ws)
+        at = 0
+        for b in range(3):
+            s = slice(done[b] - portion[b], done[b])
+            close(out[at:at + portion[b]], bounds[b][0][s], bounds[b][1][s], f"portion of {b}")
+            at += portion[b]
+    # single tokens, captured
+    sq, sk, sv = (torch.zeros(3, n, D, dtype=dtype, device=gpu) for n in (H, KH, KH))
+    spos, slen, sslots = (torch.zeros(3, dtype=torch.int32, device=gpu) for _ in range(3))
+    soff, sout, ws = offsets_of([1, 1, 1], gpu), torch.zeros(3, H, D, dtype=dtype, device=gpu), ops.attn_paged_workspace(H, KH, D, 3, gpu)
+
+    def step():
+        ops.rope_store(sq, sk, sv, spos, table, mode, kc, vc, sslots)
+        ops.attn_paged(sq, kc, vc, pages, slen, soff, sout, ws, max_new=1)
+
+    graph = None
+    for i in range(steps):
+        for b in range(3):
+            sq[b], sk[b], sv[b] = raw[b][0][done[b]], raw[b][1][done[b]], raw[b][2][done[b]]
+        spos.copy_(torch.tensor(done, dtype=torch.int32))
+        slen.copy_(spos + 1)
+        sslots.copy_(pages[torch.arange(3, device=gpu), spos.long() // page] * page + spos % page)
+        if i == 0:
+            keep = [t.clone() for t in (sq, sk)]
+            step()
+            torch.cuda.synchronize()
+            eager = sout.clone()
+            sq.copy_(keep[0])
+            sout.zero_()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+            graph.replay()
+            assert torch.equal(sout, eager)
+        else:
+            sout.fill_(math.nan)
+            torch.cuda.synchronize()
+            graph.replay()
+        for b in range(3):
+            close(sout[b:b + 1], bounds[b][0][done[b]:done[b] + 1], bounds[b][1][done[b]:done[b] + 1], f"step {i} of {b}")
+        done = [n + 1 for n in done]
+
+
+def test_another_stream_and_the_same_answer_twice(gpu):
+    from kuiperllama_amd import ops
+    gen = generator(12)
+    kc, vc, table, ks, vs = paged(gen, BF16, 2, 128, 128, [3000, 5, 800], 64)
+    q = rnd(gen, BF16, 3, 8, 128)
+    lengths, off = torch.tensor([3000, 5, 800], dtype=torch.int32, device=gpu), offsets_of([1, 1, 1], gpu)
+    ws = [ops.attn_paged_workspace(8, 2, 128, 3, gpu) for _ in range(2)]
+    outs = [torch.zeros(3, 8, 128, dtype=BF16, device=gpu) for _ in range(2)]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i in range(2):
+            with torch.cuda.stream(side[i]):
+                ops.attn_paged(q, kc, vc, table, lengths, off, outs[i], ws[i])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1])
+    check_paged(q, outs[0], [3000, 5, 800], [1, 1, 1], ks, vs, 0)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A cache of more than 4 GiB: pages at its end."""
+    from kuiperllama_amd import ops
+    pages, page, KH, D = 70000, 256, 1, 128
+    kc = torch.zeros(pages, page, KH, D, dtype=BF16, device=gpu)  # 4.6 GB
+    vc = torch.zeros(pages, page, KH, D, dtype=BF16, device=gpu)
+    gen = generator(9)
+    ids = [69999, 3, 65536, 69998]
+    n = 1000
+    k, v = rnd(gen, BF16, n, KH, D), rnd(gen, BF16, n, KH, D)
+    slots = torch.tensor([ids[j // page] * page + j % page for j in range(n)], dtype=torch.int32, device=gpu)
+    q = rnd(gen, BF16, n, 4, D)
+    table = ops.rope_table(0, 1e4, gpu)  # nothing turns
+    ops.rope_store(q, k, v, torch.zeros(n, dtype=torch.int32, device=gpu), table, 0, kc, vc, slots)
+    assert torch.equal(kc[69998, :n - 768], k[768:]) and torch.equal(vc[69999], v[:256])
+    ws = ops.attn_paged_workspace(4, KH, D, n, gpu)
+    out = torch.empty(n, 4, D, dtype=BF16, device=gpu)
+    args = (kc, vc, torch.tensor([ids], dtype=torch.int32, device=gpu), torch.tensor([n], dtype=torch.int32, device=gpu))
+    ops.attn_paged(q, *args, offsets_of([n], gpu), out, ws)
+    want, bound = attended(q, k, v, 0, D ** -0.5)
+    close(out, want, bound)
+    ops.attn_paged(q[-1:], *args, offsets_of([1], gpu), out[-1:], ws)
+    close(out[-1:], want[-1:], bound[-1:])
+
+
+def test_refusals_on_the_device(gpu):
+    from kuiperllama_amd import _ffi, ops
+    f = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device=gpu)  # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=gpu)  # noqa: E731
+    table = ops.rope_table(64, 1e4, gpu)
+    ok = dict(q=f(4, 4, 64), k=f(4, 2, 64), positions=i(4), table=table, mode=1)
+    for bad, error in ((dict(q=f(4, 4, 64, dtype=torch.float16)), TypeError), (dict(k=f(4, 2, 64, dtype=F32)), TypeError), (dict(k=f(3, 2, 64)), ValueError),
+                       (dict(k=f(4, 2, 128)), ValueError), (dict(positions=i(3)), ValueError), (dict(positions=f(4, dtype=F32)), TypeError),
+                       (dict(q_out=f(4, 4, 32)), ValueError), (dict(q=f(4, 64, 4).transpose(1, 2)), ValueError), (dict(mode=5), _ffi.KhError),
+                       (dict(q=f(4, 4, 65)[..., 1:]), _ffi.KhError), (dict(k=f(4, 3, 64)), _ffi.KhError), (dict(positions=torch.zeros(4, dtype=torch.int32)), ValueError),
+                       (dict(q=f(4, 256)), ValueError)):
+        with pytest.raises(error):
+            ops.rope_tokens(**{**ok, **bad})
+    ok = dict(q=f(4, 4, 64), kcache=f(3, 16, 2, 64), vcache=f(3, 16, 2, 64), pages=i(2, 3), lengths=i(2), offsets=i(3), out=f(4, 4, 64),
+              workspace=ops.attn_paged_workspace(4, 2, 64, 4, gpu))
+    for bad, error in ((dict(lengths=i(3)), ValueError), (dict(pages=i(3, 3)), ValueError), (dict(pages=i(2, 3).long()), ValueError), (dict(out=f(4, 4, 32)), ValueError),
+                       (dict(vcache=f(3, 8, 2, 64)), ValueError), (dict(kcache=f(3, 16, 2, 32)), ValueError), (dict(workspace=f(0).to(torch.uint8)), _ffi.KhError),
+                       (dict(scale=0.0), _ffi.KhError), (dict(kcache=f(3, 16, 2, 64, dtype=F32)), TypeError), (dict(offsets=i(3).long()), TypeError),
+                       (dict(workspace=torch.zeros(1 << 20, dtype=torch.uint8)), ValueError), (dict(max_new=-1), _ffi.KhError)):
+        with pytest.raises(error):
+            ops.attn_paged(**{**ok, **bad})
+    assert (ops.attn_paged(**ok) == 0).all()  # offsets and lengths of zero
+    ok = dict(q=f(4, 4, 64), k=f(4, 2, 64), v=f(4, 2, 64), offsets=i(2), out=f(4, 4, 64))
+    for bad, error in ((dict(k=f(3, 2, 64)), ValueError), (dict(v=f(4, 1, 64)), ValueError), (dict(v=f(4, 2, 64, dtype=F32)), TypeError), (dict(out=f(4, 4, 64, dtype=F32)), TypeError),
+                       (dict(k=f(4, 3, 64), v=f(4, 3, 64)), _ffi.KhError), (dict(q=f(4, 4, 320), k=f(4, 2, 320)), _ffi.KhError)):
+        with pytest.raises(error):
+            ops.attn_packed(**{**ok, **bad})
