@@ -104,6 +104,13 @@ __device__ __forceinline__ X lds_read(unsigned addr) {
   return *(const __attribute__((address_space(3))) X*)(size_t)addr;
 }
 
+// The same number, but nothing made of it is kept in registers over a loop
+template <bool YES>
+__device__ __forceinline__ int seq_fresh(int x) {
+  if (YES) asm volatile("" : "+v"(x));
+  return x;
+}
+
 // The running state of 32 query rows, a lane's row being l & 31.
 template <class T, int DP>
 struct SeqState {
@@ -125,7 +132,7 @@ struct SeqState {
   }
   __device__ __forceinline__ frag query(int b, int half) const {
     frag f;
-    const int c = 2 * b + half;
+    const int c = 2 * b + seq_fresh<C::TIGHT>(half);
     if (c < chunks) f = *(const frag*)(row + 16 * c);
     else
 #pragma unroll
@@ -281,7 +288,7 @@ __device__ __forceinline__ void seq_stage(const SeqArgs& a, SeqKeys& x, int k0, 
   static_assert(NL * 64 * WAVES == BN * C::CB, "whole requests");
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
-    const int i = (WAVES * j + wave) * 64 + lane, r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+    const int i = (WAVES * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
     int place = k0 + r;
     place = place < x.lo ? x.lo : (place >= x.hi ? x.hi - 1 : place);
     int64_t ko, vo;
@@ -371,6 +378,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqA
   const int b = __builtin_amdgcn_readfirstlane(seq_of_slot(a, slot, S::BM, lane));
   const SeqSpan sp = seq_span(a, b);
   const int rows = sp.n * a.group;
+  if (PAGED && rows <= 32) return;  // k_seq_rows
   const int tiles = (rows + S::BM - 1) / S::BM, tile = tiles - 1 - (slot - seq_slot_base(a, b, S::BM));
   if (tile < 0 || tile >= tiles) return;
   auto place_of = [&](int r) __attribute__((always_inline)) { return sp.length - sp.n + (r < rows ? r : rows - 1) / a.group; };
@@ -438,6 +446,329 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqA
       seq_one<T, PAGED>(a, x, a.q + (sp.first + tk) * a.q_token + hd * a.q_head, a.out + (sp.first + tk) * a.o_token + hd * a.o_head,
                         place_of(r), lane);
     }
+  }
+}
+
+// ---- few rows a sequence ---------------------------------------------------------------------------------------------------------
+// Sequences of up to 32 query rows (single tokens above all) read their keys once, whatever is done: HBM bounds them, so all keys
+// of all sequences are dealt evenly to the workgroups that fit on the chip at once.  A unit is a key head of a sequence; units lie one
+// behind the other, each a number of steps of 128 keys, and workgroup i takes steps [i W / N, (i + 1) W / N) of the W, the
+// end of one unit and the beginning of the next where they fall so.  What it finds of a unit that another has a part of goes to
+// the workspace, fp32 and with its m and l, and k_seq_join adds the parts.  Every workgroup finds its share from the lengths on the device
+// by one sum over the sequences: no table from the host, and a captured launch follows the lengths.
+struct SeqRowsArgs {
+  SeqArgs s;
+  float* ws;      // [2 N][32][value size + 2]: the part of a unit that began before workgroup i's share, the part of one that ends behind it
+  int shares, all;  // N; all: sequences of more than 32 rows too, 32 at a time
+};
+struct SeqUnits {
+  SeqSpan sp;
+  int rows, blocks, lo, hi, t0, steps;  // of each of blocks * kv_heads units
+};
+constexpr int SEQ_STEP = 128;  // four waves of 32 keys
+__device__ __forceinline__ SeqUnits seq_units(const SeqRowsArgs& a, int b) {
+  SeqUnits u;
+  u.sp = seq_span(a.s, b);
+  u.rows = u.sp.n * a.s.group;
+  u.blocks = u.rows <= 32 || a.all ? (u.rows + 31) / 32 : 0;
+  const int first = u.sp.length - u.sp.n;
+  u.lo = a.s.window > 0 && first >= a.s.window ? first - a.s.window + 1 : 0;
+  u.hi = u.sp.length;
+  u.t0 = u.lo / SEQ_STEP;
+  const int n = (u.hi + SEQ_STEP - 1) / SEQ_STEP - u.t0;
+  u.steps = n > 1 ? n : 1;  // no key at all: a step that writes the zeros
+  return u;
+}
+// Steps ahead of each sequence and in all, for a workgroup of 256.  A thread sums `per` sequences that lie side by side.
+struct SeqScan {
+  int64_t before, mine, total;  // of this thread's sequences
+  int per;
+};
+__device__ __forceinline__ SeqScan seq_scan(const SeqRowsArgs& a, int64_t* red /* [4] */) {
+  SeqScan r;
+  r.per = (a.s.n_seqs + 255) / 256;
+  r.mine = 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = (int)threadIdx.x * r.per;
+  for (int b = b0; b < b0 + r.per && b < a.s.n_seqs; ++b) {
+    const SeqUnits u = seq_units(a, b);
+    r.mine += (int64_t)u.blocks * a.s.kv_heads * u.steps;
+  }
+  int64_t x = r.mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t y = __shfl_up((long long)x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) red[wave] = x;
+  __syncthreads();
+  r.before = x - r.mine;
+  r.total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) r.before += red[w];
+    r.total += red[w];
+  }
+  return r;
+}
+// Of N workgroups, those that have work, and where the share of one begins.
+__device__ __forceinline__ int seq_shares(int64_t total, int n) { return total < n ? (int)total : n; }
+__device__ __forceinline__ int64_t seq_share(int64_t total, int n, int i) { return total * i / n; }
+__device__ __forceinline__ int seq_owner(int64_t total, int n, int64_t step) { return (int)(((step + 1) * n - 1) / total); }
+
+template <class T, int DP>
+struct SeqRows {
+  typedef SeqCfg<T, DP> C;
+  static constexpr int TB = 32 * C::RB;  // keys of a wave's tile, or their values
+  // A wave has a ring of such halves of its own: keys, values, keys ..., as many as leave the CU its other waves
+  static constexpr int NB = C::RB <= 256 ? 4 : (C::RB == 512 ? 2 : 1);
+  static constexpr int NL = 32 * C::CB / 64;  // requests for one
+  static constexpr int PITCH = DP + 1;        // of a row of partial outputs, in the same place
+  static constexpr int RING = 4 * NB * TB > 16 * 32 * PITCH ? 4 * NB * TB : 16 * 32 * PITCH;
+  static constexpr int TAB = 1024;  // pages looked up at once
+  static constexpr int LDS = RING + 4 * TAB + 1024 + 64;
+};
+
+// The final rows of a unit: o / l, and with care where that is no number.
+template <class T>
+__device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, int b, int head, int r0, int rows, bool odd, int wave, int lane) {
+  if (!odd) return;
+  for (int r = r0 + wave; r < r0 + rows; r += 4) {
+    const int tk = r / a.group, h = head * a.group + r - tk * a.group, place = u.sp.length - u.sp.n + tk;
+    SeqKeys x = seq_keys(a, b, head, u.sp, place, place);
+    seq_one<T, true>(a, x, a.q + (u.sp.first + tk) * a.q_token + h * a.q_head, a.out + (u.sp.first + tk) * a.o_token + h * a.o_head, place, lane);
+  }
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, (SeqCfg<T, DP>::RB <= 128 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs ra) {
+  typedef SeqRows<T, DP> S;
+  typedef SeqCfg<T, DP> C;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  int* tab = (int*)(smem_raw + S::RING);
+  float *ms = (float*)(tab + S::TAB), *ls = ms + 128;
+  int64_t* red = (int64_t*)(ls + 128);
+  int* flag = (int*)(red + 4);
+  const SeqArgs& a = ra.s;
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
+  const unsigned ring = lds0 + (unsigned)(wave * S::NB * S::TB);
+  // ---- this workgroup's share
+  const SeqScan sc = seq_scan(ra, red);
+  const int n_shares = seq_shares(sc.total, ra.shares), share = blockIdx.x;
+  if (share >= n_shares) return;
+  int64_t at = seq_share(sc.total, n_shares, share);
+  const int64_t end = seq_share(sc.total, n_shares, share + 1);
+  if (sc.before <= at && at < sc.before + sc.mine) {  // one thread
+    int64_t p = sc.before;
+    int b = (int)threadIdx.x * sc.per;
+    for (;; ++b) {
+      const SeqUnits u = seq_units(ra, b);
+      const int64_t n = (int64_t)u.blocks * a.kv_heads * u.steps;
+      if (at < p + n) break;
+      p += n;
+    }
+    flag[0] = b;
+    *(int64_t*)(flag + 2) = p;
+  }
+  __syncthreads();
+  int b = __builtin_amdgcn_readfirstlane(flag[0]);
+  int64_t ahead = *(int64_t*)(flag + 2);  // steps ahead of sequence b
+  SeqUnits u = seq_units(ra, b);
+  while (at < end) {
+    while (at >= ahead + (int64_t)u.blocks * a.kv_heads * u.steps) {
+      ahead += (int64_t)u.blocks * a.kv_heads * u.steps;
+      u = seq_units(ra, ++b);
+    }
+    const int unit = (int)((at - ahead) / u.steps), ta = (int)((at - ahead) - (int64_t)unit * u.steps);
+    const int tb = u.steps - ta < end - at ? u.steps : ta + (int)(end - at);
+    at += tb - ta;
+    const int head = unit / u.blocks, r0 = 32 * (unit - head * u.blocks);
+    const int n_rows = u.rows - r0 < 32 ? u.rows - r0 : 32;
+    const int row = r0 + ((lane & 31) < n_rows ? (lane & 31) : n_rows - 1);
+    const int token = row / a.group, h = head * a.group + row - token * a.group, place = u.sp.length - u.sp.n + token;
+    const int first_place = u.sp.length - u.sp.n + r0 / a.group, last_place = u.sp.length - u.sp.n + (r0 + n_rows - 1) / a.group;
+    SeqKeys x = seq_keys(a, b, head, u.sp, u.sp.length - u.sp.n, u.sp.length - 1);
+    SeqState<T, DP> st;
+    st.load_q(a.q + (u.sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
+    st.clear();
+    if (threadIdx.x == 0) flag[1] = x.bad;
+    const int per_table = (S::TAB - 1) * (int64_t)a.kv.page_size / SEQ_STEP < 1 << 20 ? (int)((S::TAB - 1) * (int64_t)a.kv.page_size / SEQ_STEP) : 1 << 20;
+    for (int c0 = ta; c0 < tb && u.hi > u.lo; c0 += per_table) {
+      const int c1 = tb - c0 < per_table ? tb : c0 + per_table;
+      // pages of these steps
+      const int ka = (u.t0 + c0) * SEQ_STEP > u.lo ? (u.t0 + c0) * SEQ_STEP : u.lo, kb = (u.t0 + c1) * SEQ_STEP < u.hi ? (u.t0 + c1) * SEQ_STEP : u.hi;
+      auto page_of = [&](int k) __attribute__((always_inline)) { return a.kv.magic ? (int)(__umulhi((uint32_t)k, a.kv.magic) >> a.kv.shift) : k; };
+      const int p0 = page_of(ka), np = page_of(kb - 1) - p0 + 1;
+      __syncthreads();  // the table before, and partial outputs, are read
+      for (int i = threadIdx.x; i < np; i += 256) {
+        const int page = x.table[p0 + i];
+        const bool ok = (unsigned)page < (unsigned)a.kv.n_pages;
+        tab[i] = ok ? page : 0;
+        if (!ok) flag[1] = 1;
+      }
+      __syncthreads();
+      // half h of these steps: the keys (h even) or the values of step h / 2
+      const int halves = 2 * (c1 - c0);
+      auto issue = [&](int h) __attribute__((always_inline)) {
+        const int k0 = (u.t0 + c0 + (h >> 1)) * SEQ_STEP + 32 * wave;
+        const unsigned dst = ring + (unsigned)(h % S::NB * S::TB);
+        const bool keys = (h & 1) == 0;
+        const char* base = keys ? x.k : x.v;
+        const int64_t ps = keys ? a.kv.k_page : a.kv.v_page, ss = keys ? a.kv.k_slot : a.kv.v_slot;
+        const int chunks = keys ? a.kchunks : a.vchunks;
+#pragma unroll
+        for (int j = 0; j < S::NL; ++j) {
+          const int i = j * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+          int key = k0 + r;
+          key = key < ka ? ka : (key >= kb ? kb - 1 : key);
+          const int p = page_of(key), sl = key - p * a.kv.page_size, page = tab[p - p0];
+          dma_x4_from(c < chunks ? base + page * ps + sl * ss + 16 * c : (const char*)&seq_zeros, dst + 1024 * j);
+          if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto landed = [&](int h) __attribute__((always_inline)) {
+        const int behind = halves - 1 - h;
+        if (S::NB > 3 && behind >= 3) wait_vm<(S::NB > 3 ? 3 : 0) * S::NL>();
+        else if (S::NB > 2 && behind >= 2) wait_vm<(S::NB > 2 ? 2 : 0) * S::NL>();
+        else if (S::NB > 1 && behind >= 1) wait_vm<(S::NB > 1 ? 1 : 0) * S::NL>();
+        else wait_vm<0>();
+      };
+      auto used = [&](int h) __attribute__((always_inline)) {
+        if (h + S::NB < halves) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // half h is read
+          issue(h + S::NB);
+        }
+      };
+      for (int h = 0; h < S::NB && h < halves; ++h) issue(h);
+      for (int t = c0; t < c1; ++t) {
+        const int h = 2 * (t - c0), k0 = (u.t0 + t) * SEQ_STEP + 32 * wave;
+        const bool some = k0 < kb && k0 + 32 > ka;
+        f32x16 s;
+        landed(h);
+        if (some) {
+          s = st.scores(ring + (unsigned)(h % S::NB * S::TB), 0, lane);
+        }
+        used(h);
+        if (some) {
+          if (k0 + 31 > first_place || (a.window > 0 && k0 <= last_place - a.window)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int back = place - (k0 + 8 * (i >> 2) + 4 * half + (i & 3));
+              if (back < 0 || (a.window > 0 && back >= a.window)) s[i] = -INFINITY;
+            }
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+          st.follow(xor32_max(mx), a.c);
+          s = st.weigh(s, a.c);
+        }
+        landed(h + 1);
+        if (some) st.add(s, ring + (unsigned)((h + 1) % S::NB * S::TB), 0, lane);
+        used(h + 1);
+      }
+    }
+    // ---- the four waves' sums
+    const float l = xor32_sum(st.l);
+    if (half == 0) {
+      ms[32 * wave + lane] = st.m;
+      ls[32 * wave + lane] = l;
+    }
+    __syncthreads();  // everyone is done with the ring
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[32 * w + (lane & 31)]);
+    const float f = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m - m) * a.c);
+    float* part = (float*)smem_raw;
+    if ((lane & 31) < n_rows) {
+#pragma unroll
+      for (int n = 0; n < C::NMB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(32 * wave + (lane & 31)) * S::PITCH + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3)] = st.o[n][i] * f;
+    }
+    __syncthreads();
+    const bool bad = flag[1] != 0;
+    const int cols = a.vchunks * C::E;
+    const bool whole = ta == 0 && tb == u.steps;
+    float* ws = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 2);
+    bool odd = false;
+    for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
+      const int r = e / cols, d = e - r * cols;
+      float mr = -INFINITY, lr = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mr = fmaxf(mr, ms[32 * w + r]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = ms[32 * w + r];
+        lr += mw == -INFINITY ? ls[32 * w + r] : ls[32 * w + r] * __builtin_amdgcn_exp2f((mw - mr) * a.c);
+        o += part[(32 * w + r) * S::PITCH + d];
+      }
+      if (bad) lr = NAN;
+      if (whole) {
+        const float v = lr == 0.f ? 0.f : o / lr;
+        odd |= !(fabsf(v) < INFINITY);
+        const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+        ((T*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head))[d] = (T)v;
+      } else {
+        ws[r * (cols + 2) + d] = o;
+        if (d == 0) {
+          ws[r * (cols + 2) + cols] = mr;
+          ws[r * (cols + 2) + cols + 1] = lr;
+        }
+      }
+    }
+    odd = __syncthreads_or(odd);
+    if (whole) seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
+  }
+}
+
+// Units that several workgroups had a part of.  grid (n_seqs * kv_heads)
+template <class T>
+__global__ __launch_bounds__(256) void k_seq_join(const SeqRowsArgs ra) {
+  __shared__ int64_t red[4];
+  __shared__ int64_t ahead_of;
+  const SeqArgs& a = ra.s;
+  const int b = (int)blockIdx.x / a.kv_heads, head = (int)blockIdx.x - b * a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const SeqScan sc = seq_scan(ra, red);
+  const SeqUnits u = seq_units(ra, b);
+  if (u.blocks == 0) return;
+  if ((int)threadIdx.x == b / sc.per) {
+    int64_t p = sc.before;
+    for (int i = (int)threadIdx.x * sc.per; i < b; ++i) {
+      const SeqUnits v = seq_units(ra, i);
+      p += (int64_t)v.blocks * a.kv_heads * v.steps;
+    }
+    ahead_of = p;
+  }
+  __syncthreads();
+  const int n_shares = seq_shares(sc.total, ra.shares), cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 2;
+  for (int k = 0; k < u.blocks; ++k) {
+    const int64_t s0 = ahead_of + (int64_t)(head * u.blocks + k) * u.steps;
+    const int i0 = seq_owner(sc.total, n_shares, s0), i1 = seq_owner(sc.total, n_shares, s0 + u.steps - 1);
+    if (i0 == i1) continue;
+    const int r0 = 32 * k, n_rows = u.rows - r0 < 32 ? u.rows - r0 : 32;
+    bool odd = false;
+    for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
+      const int r = e / cols, d = e - r * cols;
+      const float* first = ra.ws + ((size_t)(2 * i0 + 1) * 32 + r) * pitch;
+      const float* rest = ra.ws + ((size_t)(2 * i0 + 2) * 32 + r) * pitch;  // of workgroup i0 + 1
+      const size_t next = (size_t)2 * 32 * pitch;
+      float m = first[cols];
+      for (int i = 0; i < i1 - i0; ++i) m = fmaxf(m, rest[i * next + cols]);
+      float l = 0.f, o = 0.f;
+      for (int i = -1; i < i1 - i0; ++i) {
+        const float* w = i < 0 ? first : rest + i * next;
+        const float f = w[cols] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w[cols] - m) * a.c);
+        l += w[cols] == -INFINITY ? w[cols + 1] : w[cols + 1] * f;  // NaN of a page that is none
+        o += w[d] * f;
+      }
+      const float v = l == 0.f ? 0.f : o / l;
+      odd |= !(fabsf(v) < INFINITY);
+      const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+      ((T*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head))[d] = (T)v;
+    }
+    odd = __syncthreads_or(odd);
+    seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
   }
 }
 }  // namespace khm

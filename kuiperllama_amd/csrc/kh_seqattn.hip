@@ -48,8 +48,8 @@ SeqArgs args_of(const kh_attn_rows* r, int e) {
   return a;
 }
 
-template <class K>
-int launch(K kern, unsigned grid, int threads, int lds, const SeqArgs& a, hipStream_t s) {
+template <class K, class A>
+int launch(K kern, unsigned grid, int threads, int lds, const A& a, hipStream_t s) {
   if (lds > 64 * 1024) KH_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
   hipLaunchKernelGGL(kern, dim3(grid), dim3(threads), lds, s, a);
   return kh_launch_status();
@@ -62,11 +62,25 @@ int tiles(const SeqArgs& a, hipStream_t s) {
   return launch(k_seq_tiles<T, DP, PAGED>, (unsigned)(slots * a.kv_heads), 64 * S::W, S::LDS, a, s);
 }
 
+constexpr int SHARES = 512;  // workgroups of k_seq_rows: two on each of MI355X's 256 CUs
+
+template <class T, int DP>
+int rows(const SeqRowsArgs& a, hipStream_t s) {
+  const int rc = launch(k_seq_rows<T, DP>, SHARES, 256, SeqRows<T, DP>::LDS, a, s);
+  return rc != KH_OK ? rc : launch(k_seq_join<T>, (unsigned)(a.s.n_seqs * a.s.kv_heads), 256, 0, a, s);
+}
+
 template <bool PAGED>
 int go(const SeqArgs& a, int e, hipStream_t s) {
   const int most = (a.kchunks > a.vchunks ? a.kchunks : a.vchunks) * 16 / e;
   if (e == 2) return most <= 64 ? tiles<bf16, 64, PAGED>(a, s) : (most <= 128 ? tiles<bf16, 128, PAGED>(a, s) : tiles<bf16, 256, PAGED>(a, s));
   return most <= 64 ? tiles<float, 64, PAGED>(a, s) : (most <= 128 ? tiles<float, 128, PAGED>(a, s) : tiles<float, 256, PAGED>(a, s));
+}
+
+int go_rows(const SeqRowsArgs& a, int e, hipStream_t s) {
+  const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
+  if (e == 2) return most <= 64 ? rows<bf16, 64>(a, s) : (most <= 128 ? rows<bf16, 128>(a, s) : rows<bf16, 256>(a, s));
+  return most <= 64 ? rows<float, 64>(a, s) : (most <= 128 ? rows<float, 128>(a, s) : rows<float, 256>(a, s));
 }
 }  // namespace
 }  // namespace khm
@@ -91,7 +105,7 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
 
 extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
   if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
-  return 16;
+  return (int64_t)2 * khm::SHARES * 32 * (value_size + 2) * 4;
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
@@ -129,5 +143,12 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
   a.kv.magic = c->page_size == 1 ? 0 : (uint32_t)((1ull << (31 + bits)) / (uint64_t)c->page_size + 1);
   a.kv.shift = bits - 1;
   a.kv.lengths = lengths;
-  return khm::go<true>(a, e, (hipStream_t)stream);
+  // rows of a sequence: one with more than 32 has tiles of its own
+  const int64_t most = (int64_t)(max_new && max_new < r->n_tokens ? max_new : r->n_tokens) * a.group;
+  if (most > 32) {
+    const int done = khm::go<true>(a, e, (hipStream_t)stream);
+    if (done != KH_OK) return done;
+  }
+  khm::SeqRowsArgs ra{a, (float*)workspace, khm::SHARES, most <= 32};
+  return khm::go_rows(ra, e, (hipStream_t)stream);
 }
