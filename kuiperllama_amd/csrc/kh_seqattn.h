@@ -453,19 +453,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqA
 // Sequences of up to 32 query rows (single tokens above all) read their keys once, whatever is done: HBM bounds them, so all keys
 // of all sequences are dealt evenly to the workgroups that fit on the chip at once.  A unit is a key head of a sequence; units lie one
 // behind the other, each a number of steps of 128 keys, and workgroup i takes steps [i W / N, (i + 1) W / N) of the W, the
-// end of one unit and the beginning of the next where they fall so.  What it finds of a unit that another has a part of goes to
-// the workspace, fp32 and with its m and l, and k_seq_join adds the parts.  Every workgroup finds its share from the lengths on the device
-// by one sum over the sequences: no table from the host, and a captured launch follows the lengths.
+// end of one unit and the beginning of the next where they fall so.  What it finds of a unit that others have parts of goes to
+// the workspace, fp32 and with its m and l; the workgroup that is the last to bring a part adds them, in the order of the keys whoever
+// it is.  Every workgroup finds its share from the lengths on the device by one sum over the sequences: no table from the host, and a
+// captured launch follows the lengths.
 struct SeqRowsArgs {
   SeqArgs s;
-  float* ws;      // [2 N][32][value size + 2]: the part of a unit that began before workgroup i's share, the part of one that ends behind it
+  // [N] parts brought of the unit that begins in workgroup i's share and ends behind it, 0 between launches
+  int* brought;
+  float* ws;        // [2 N][32][value size + 4], o, m, l: of the unit that began before workgroup i's share, of the one that ends behind it
   int shares, all;  // N; all: sequences of more than 32 rows too, 32 at a time
 };
 struct SeqUnits {
   SeqSpan sp;
   int rows, blocks, lo, hi, t0, steps;  // of each of blocks * kv_heads units
 };
-constexpr int SEQ_STEP = 128;  // four waves of 32 keys
+constexpr int SEQ_STEP = 128;     // four waves of 32 keys
+constexpr int SEQ_SHARES = 512;   // the most: two workgroups on each of MI355X's 256 CUs
 __device__ __forceinline__ SeqUnits seq_units(const SeqRowsArgs& a, int b) {
   SeqUnits u;
   u.sp = seq_span(a.s, b);
@@ -520,12 +524,14 @@ struct SeqRows {
   typedef SeqCfg<T, DP> C;
   static constexpr int TB = 32 * C::RB;  // keys of a wave's tile, or their values
   // A wave has a ring of such halves of its own: keys, values, keys ..., as many as leave the CU its other waves
-  static constexpr int NB = C::RB <= 256 ? 4 : (C::RB == 512 ? 2 : 1);
+  static constexpr int NB = C::RB <= 128 ? 4 : (C::RB <= 512 ? 2 : 1);
   static constexpr int NL = 32 * C::CB / 64;  // requests for one
   static constexpr int PITCH = DP + 1;        // of a row of partial outputs, in the same place
   static constexpr int RING = 4 * NB * TB > 16 * 32 * PITCH ? 4 * NB * TB : 16 * 32 * PITCH;
   static constexpr int TAB = 1024;  // pages looked up at once
   static constexpr int LDS = RING + 4 * TAB + 1024 + 64;
+  static_assert(32 * SEQ_SHARES * 4 <= RING && 4096 <= 4 * TAB, "the parts' weights fit the ring, their sums the table");
+  static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
 };
 
 // The final rows of a unit: o / l, and with care where that is no number.
@@ -539,8 +545,77 @@ __device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, 
   }
 }
 
+// Partial results pass between workgroups, maybe of different XCDs, in agent-scope words, which are stored through and read past the
+// caches that are not common: with 512 workgroups, a fence for each part costs the launch 15 - 20 us.
+__device__ __forceinline__ void seq_give(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float seq_take(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The rows of a unit from its parts: their weights (LDS, [32][parts]), then their outputs, four columns a thread and as many parts side by
+// side as there are threads.  True where an output is no number.
+template <class T>
+__device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& u, int head, int r0, int n_rows, int i0, int parts, float* weight,
+                                         float* ls, f32x4* red, int wave, int lane) {
+  const SeqArgs& a = ra.s;
+  const int cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 4;
+  // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
+  auto at = [&](int r, int p) __attribute__((always_inline)) { return ra.ws + ((size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 32 + r) * pitch; };
+  for (int r = wave; r < n_rows; r += 4) {
+    float m = -INFINITY, l = 0.f;
+    for (int p = lane; p < parts; p += 64) m = fmaxf(m, seq_take(at(r, p) + cols));
+    m = wave_max(m);
+    for (int p = lane; p < parts; p += 64) {
+      const float mp = seq_take(at(r, p) + cols), lp = seq_take(at(r, p) + cols + 1);
+      const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
+      weight[r * parts + p] = f;
+      l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
+    }
+    l = wave_sum(l);
+    if (lane == 0) ls[r] = l;
+  }
+  __syncthreads();
+  int across = 1, down = 1;  // threads of a row: its columns by four; rows at once
+  while (across * 4 < cols) across *= 2;
+  while (down < n_rows && down * across < 256) down *= 2;
+  const int side = 256 / (across * down), x = (int)threadIdx.x & (across - 1), y = (int)threadIdx.x / across & (down - 1),
+            z = (int)threadIdx.x / (across * down);
+  bool odd = false;
+  for (int rb = 0; rb < n_rows; rb += down) {
+    const int r = rb + y;
+    const bool mine = r < n_rows && 4 * x < cols;
+    f32x4 o = f4_zero();
+    if (mine) {
+#pragma unroll 4
+      for (int p = z; p < parts; p += side) {
+        const float* v = at(r, p) + 4 * x;
+        const float f = weight[r * parts + p];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(seq_take(v + i), f, o[i]);
+      }
+    }
+    red[threadIdx.x] = o;
+    __syncthreads();
+    if (mine && z == 0) {
+      for (int p = 1; p < side && p < parts; ++p) {
+        const f32x4 v = red[p * across * down + threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += v[i];
+      }
+      const float l = ls[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = l == 0.f ? 0.f : o[i] / l;
+        odd |= !(fabsf(o[i]) < INFINITY);
+      }
+      const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+      *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + 4 * x * (int)sizeof(T)) = to_quad<T>(o);
+    }
+    __syncthreads();
+  }
+  return odd;
+}
+
 template <class T, int DP>
-__global__ __launch_bounds__(256, (SeqCfg<T, DP>::RB <= 128 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs ra) {
+__global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs ra) {
   typedef SeqRows<T, DP> S;
   typedef SeqCfg<T, DP> C;
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
@@ -618,7 +693,7 @@ __global__ __launch_bounds__(256, (SeqCfg<T, DP>::RB <= 128 ? 2 : 1)) void k_seq
         const int chunks = keys ? a.kchunks : a.vchunks;
 #pragma unroll
         for (int j = 0; j < S::NL; ++j) {
-          const int i = j * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+          const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
           int key = k0 + r;
           key = key < ka ? ka : (key >= kb ? kb - 1 : key);
           const int p = page_of(key), sl = key - p * a.kv.page_size, page = tab[p - p0];
@@ -690,7 +765,7 @@ __global__ __launch_bounds__(256, (SeqCfg<T, DP>::RB <= 128 ? 2 : 1)) void k_seq
     const bool bad = flag[1] != 0;
     const int cols = a.vchunks * C::E;
     const bool whole = ta == 0 && tb == u.steps;
-    float* ws = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 2);
+    float* ws = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4);
     bool odd = false;
     for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
       const int r = e / cols, d = e - r * cols;
@@ -710,65 +785,29 @@ __global__ __launch_bounds__(256, (SeqCfg<T, DP>::RB <= 128 ? 2 : 1)) void k_seq
         const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
         ((T*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head))[d] = (T)v;
       } else {
-        ws[r * (cols + 2) + d] = o;
+        seq_give(ws + r * (cols + 4) + d, o);
         if (d == 0) {
-          ws[r * (cols + 2) + cols] = mr;
-          ws[r * (cols + 2) + cols + 1] = lr;
+          seq_give(ws + r * (cols + 4) + cols, mr);
+          seq_give(ws + r * (cols + 4) + cols + 1, lr);
         }
       }
     }
-    odd = __syncthreads_or(odd);
-    if (whole) seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
-  }
-}
-
-// Units that several workgroups had a part of.  grid (n_seqs * kv_heads)
-template <class T>
-__global__ __launch_bounds__(256) void k_seq_join(const SeqRowsArgs ra) {
-  __shared__ int64_t red[4];
-  __shared__ int64_t ahead_of;
-  const SeqArgs& a = ra.s;
-  const int b = (int)blockIdx.x / a.kv_heads, head = (int)blockIdx.x - b * a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const SeqScan sc = seq_scan(ra, red);
-  const SeqUnits u = seq_units(ra, b);
-  if (u.blocks == 0) return;
-  if ((int)threadIdx.x == b / sc.per) {
-    int64_t p = sc.before;
-    for (int i = (int)threadIdx.x * sc.per; i < b; ++i) {
-      const SeqUnits v = seq_units(ra, i);
-      p += (int64_t)v.blocks * a.kv_heads * v.steps;
-    }
-    ahead_of = p;
-  }
-  __syncthreads();
-  const int n_shares = seq_shares(sc.total, ra.shares), cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 2;
-  for (int k = 0; k < u.blocks; ++k) {
-    const int64_t s0 = ahead_of + (int64_t)(head * u.blocks + k) * u.steps;
-    const int i0 = seq_owner(sc.total, n_shares, s0), i1 = seq_owner(sc.total, n_shares, s0 + u.steps - 1);
-    if (i0 == i1) continue;
-    const int r0 = 32 * k, n_rows = u.rows - r0 < 32 ? u.rows - r0 : 32;
-    bool odd = false;
-    for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
-      const int r = e / cols, d = e - r * cols;
-      const float* first = ra.ws + ((size_t)(2 * i0 + 1) * 32 + r) * pitch;
-      const float* rest = ra.ws + ((size_t)(2 * i0 + 2) * 32 + r) * pitch;  // of workgroup i0 + 1
-      const size_t next = (size_t)2 * 32 * pitch;
-      float m = first[cols];
-      for (int i = 0; i < i1 - i0; ++i) m = fmaxf(m, rest[i * next + cols]);
-      float l = 0.f, o = 0.f;
-      for (int i = -1; i < i1 - i0; ++i) {
-        const float* w = i < 0 ? first : rest + i * next;
-        const float f = w[cols] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w[cols] - m) * a.c);
-        l += w[cols] == -INFINITY ? w[cols + 1] : w[cols + 1] * f;  // NaN of a page that is none
-        o += w[d] * f;
+    if (!whole) {
+      const int64_t s0 = ahead + (int64_t)unit * u.steps;
+      const int i0 = seq_owner(sc.total, n_shares, s0), parts = seq_owner(sc.total, n_shares, s0 + u.steps - 1) - i0 + 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        flag[0] = __hip_atomic_fetch_add(&ra.brought[i0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        if (flag[0]) __hip_atomic_store(&ra.brought[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
-      const float v = l == 0.f ? 0.f : o / l;
-      odd |= !(fabsf(v) < INFINITY);
-      const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
-      ((T*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head))[d] = (T)v;
+      __syncthreads();
+      if (!flag[0]) continue;
+      odd = seq_join<T>(ra, u, head, r0, n_rows, i0, parts, (float*)smem_raw, ls, (f32x4*)tab, wave, lane);
     }
     odd = __syncthreads_or(odd);
     seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
   }
 }
+
 }  // namespace khm

@@ -49,9 +49,9 @@ SeqArgs args_of(const kh_attn_rows* r, int e) {
 }
 
 template <class K, class A>
-int launch(K kern, unsigned grid, int threads, int lds, const A& a, hipStream_t s) {
+int launch(K kern, dim3 grid, int threads, int lds, const A& a, hipStream_t s) {
   if (lds > 64 * 1024) KH_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(threads), lds, s, a);
+  hipLaunchKernelGGL(kern, grid, dim3(threads), lds, s, a);
   return kh_launch_status();
 }
 
@@ -59,15 +59,13 @@ template <class T, int DP, bool PAGED>
 int tiles(const SeqArgs& a, hipStream_t s) {
   typedef SeqTiles<T, DP> S;
   const int64_t slots = (int64_t)a.n_tokens * a.group / S::BM + a.n_seqs;
-  return launch(k_seq_tiles<T, DP, PAGED>, (unsigned)(slots * a.kv_heads), 64 * S::W, S::LDS, a, s);
+  return launch(k_seq_tiles<T, DP, PAGED>, dim3((unsigned)(slots * a.kv_heads)), 64 * S::W, S::LDS, a, s);
 }
 
-constexpr int SHARES = 512;  // workgroups of k_seq_rows: two on each of MI355X's 256 CUs
-
 template <class T, int DP>
-int rows(const SeqRowsArgs& a, hipStream_t s) {
-  const int rc = launch(k_seq_rows<T, DP>, SHARES, 256, SeqRows<T, DP>::LDS, a, s);
-  return rc != KH_OK ? rc : launch(k_seq_join<T>, (unsigned)(a.s.n_seqs * a.s.kv_heads), 256, 0, a, s);
+int rows(SeqRowsArgs a, hipStream_t s) {
+  a.shares = SeqRows<T, DP>::SHARES;
+  return launch(k_seq_rows<T, DP>, dim3(a.shares), 256, SeqRows<T, DP>::LDS, a, s);
 }
 
 template <bool PAGED>
@@ -105,7 +103,7 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
 
 extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
   if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
-  return (int64_t)2 * khm::SHARES * 32 * (value_size + 2) * 4;
+  return (int64_t)khm::SEQ_SHARES * 4 + (int64_t)2 * khm::SEQ_SHARES * 32 * (value_size + 4) * 4;
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
@@ -149,6 +147,6 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
     const int done = khm::go<true>(a, e, (hipStream_t)stream);
     if (done != KH_OK) return done;
   }
-  khm::SeqRowsArgs ra{a, (float*)workspace, khm::SHARES, most <= 32};
+  khm::SeqRowsArgs ra{a, (int*)workspace, (float*)workspace + khm::SEQ_SHARES, 0, most <= 32};
   return khm::go_rows(ra, e, (hipStream_t)stream);
 }

@@ -356,11 +356,11 @@ def attn_packed(q, k, v, offsets, out, scale: Optional[float] = None, window: in
 
 
 def attn_paged_workspace(heads: int, kv_heads: int, value_size: int, tokens: int, device):
-    """Workspace of attn_paged for up to `tokens` tokens a call."""
+    """Zeroed workspace of attn_paged for up to `tokens` tokens a call."""
     n = int(_ffi.lib().kh_attn_paged_workspace_bytes(heads, kv_heads, value_size, tokens))
     if n < 0:
         _ffi.check(n, "kh_attn_paged_workspace_bytes")
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def attn_paged(q, kcache, vcache, pages, lengths, offsets, out, workspace, scale: Optional[float] = None, window: int = 0,

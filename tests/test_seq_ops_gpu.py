@@ -286,7 +286,6 @@ def test_paged(gpu, dtype, case):
     ws = ops.attn_paged_workspace(H, KH, DV, T + 2, gpu)
     for max_new in (None, max(new), 1):  # the last may be wrong: it may change no result but by the order of sums
         out = torch.full((T + 2, H, DV), 9.0, dtype=dtype, device=gpu)
-        ws.fill_(0xff)
         assert ops.attn_paged(q, kc, vc, table, lengths, offsets_of(new, gpu), out, ws, window=window, max_new=max_new) is out
         check_paged(q, out, lens, new, ks, vs, window, f"max_new {max_new}")
         assert (out[T:] == 9.0).all()
