@@ -53,7 +53,8 @@ def build_pyops(force: bool = False) -> str | None:
     """The operator calls without ctypes (csrc/kh_pyops.c): a CPython extension that needs the interpreter's headers alone.
     None, and a line on stderr, without them: the library and its models do not need it, kuiperllama_amd.ops does."""
     src = os.path.join(CSRC, "kh_pyops.c")
-    if not force and os.path.exists(PYOPS_PATH) and os.path.getmtime(src) <= os.path.getmtime(PYOPS_PATH):
+    header = os.path.join(_PKG, "..", "include", "kuiper_hip.h")
+    if not force and os.path.exists(PYOPS_PATH) and max(os.path.getmtime(src), os.path.getmtime(header)) <= os.path.getmtime(PYOPS_PATH):
         return PYOPS_PATH
     include = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(include, "Python.h")):

@@ -479,7 +479,7 @@ def test_refusals_on_the_device(gpu):
             ops.rope_tokens(**{**ok, **bad})
     ok = dict(q=f(4, 4, 64), kcache=f(3, 16, 2, 64), vcache=f(3, 16, 2, 64), pages=i(2, 3), lengths=i(2), offsets=i(3), out=f(4, 4, 64),
               workspace=ops.attn_paged_workspace(4, 2, 64, 4, gpu))
-    for bad, error in ((dict(lengths=i(3)), ValueError), (dict(pages=i(3, 3)), ValueError), (dict(pages=i(2, 3).long()), ValueError), (dict(out=f(4, 4, 32)), ValueError),
+    for bad, error in ((dict(lengths=i(3)), ValueError), (dict(pages=i(3, 3)), ValueError), (dict(pages=i(2, 3).long()), TypeError), (dict(out=f(4, 4, 32)), ValueError),
                        (dict(vcache=f(3, 8, 2, 64)), ValueError), (dict(kcache=f(3, 16, 2, 32)), ValueError), (dict(workspace=f(0).to(torch.uint8)), _ffi.KhError),
                        (dict(scale=0.0), _ffi.KhError), (dict(kcache=f(3, 16, 2, 64, dtype=F32)), TypeError), (dict(offsets=i(3).long()), TypeError),
                        (dict(workspace=torch.zeros(1 << 20, dtype=torch.uint8)), ValueError), (dict(max_new=-1), _ffi.KhError)):
