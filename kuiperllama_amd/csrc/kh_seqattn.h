@@ -280,24 +280,28 @@ __device__ __forceinline__ void seq_row(const SeqArgs& a, SeqKeys& x, int place,
     vo = place * a.kv.v_slot;
   }
 }
-// One of WAVES waves brings its part of keys k0 .. k0 + BN - 1 and their values to LDS.
-template <class T, int DP, int BN, int WAVES, bool PAGED>
-__device__ __forceinline__ void seq_stage(const SeqArgs& a, SeqKeys& x, int k0, unsigned K, unsigned V, int wave, int lane) {
-  typedef SeqCfg<T, DP> C;
-  constexpr int NL = BN * C::CB / (64 * WAVES);
-  static_assert(NL * 64 * WAVES == BN * C::CB, "whole requests");
-#pragma unroll
-  for (int j = 0; j < NL; ++j) {
-    const int i = (WAVES * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
-    int place = k0 + r;
-    place = place < x.lo ? x.lo : (place >= x.hi ? x.hi - 1 : place);
-    int64_t ko, vo;
-    seq_row<PAGED>(a, x, place, ko, vo);
-    const unsigned at = (unsigned)((WAVES * j + wave) * 1024);
-    dma_x4_from(c < a.kchunks ? x.k + ko + 16 * c : (const char*)&seq_zeros, K + at);
-    dma_x4_from(c < a.vchunks ? x.v + vo + 16 * c : (const char*)&seq_zeros, V + at);
-    if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
+__device__ __forceinline__ int seq_page(const SeqKv& kv, int place) {
+  return kv.magic ? (int)(__umulhi((uint32_t)place, kv.magic) >> kv.shift) : place;
+}
+// A sequence's pages are looked up SEQ_TAB at a time, into LDS: an address then waits for no memory, and above all not for the
+// requests under way, which a load of its own would have to let pass.
+constexpr int SEQ_TAB = 1024;
+constexpr int SEQ_SHARES = 512;  // the most that work is dealt to: two workgroups on each of MI355X's 256 CUs
+// Steps of `keys` keys that surely need no more pages than the table holds.
+__device__ __forceinline__ int seq_table_steps(const SeqKv& kv, int keys) {
+  const int64_t n = (int64_t)(SEQ_TAB - 1) * kv.page_size / keys;
+  return n < 1 << 20 ? (int)n : 1 << 20;
+}
+// The pages of keys [ka, kb); *bad where one is outside the cache.  Barriers before and after are the caller's.
+__device__ __forceinline__ int seq_table(const SeqKv& kv, const int32_t* table, int ka, int kb, int* tab, int* bad) {
+  const int p0 = seq_page(kv, ka), n = seq_page(kv, kb - 1) - p0 + 1;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int page = table[p0 + i];
+    const bool ok = (unsigned)page < (unsigned)kv.n_pages;
+    tab[i] = ok ? page : 0;
+    if (!ok) *bad = 1;
   }
+  return p0;
 }
 
 // One query by one wave from global memory, 64 keys at a time: a lane has a key for the scores, four columns for the output.  A key
@@ -363,90 +367,164 @@ struct SeqTiles {
   static constexpr int W = 4, BM = 32 * W;
   static constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   static constexpr int TB = BN * SeqCfg<T, DP>::RB;  // bytes of a tile of keys
-  static constexpr int LDS = 4 * TB;                 // two tiles of keys and values each
+  static constexpr int RING = 4 * TB;                // two tiles of keys and values each
+  static constexpr int MOST = 1024;                  // slots whose steps are dealt
+  static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
+  static constexpr int SHARES = LDS_SHARES <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
+  static constexpr int LEAST = 512 / BN;             // steps of a share
 };
 
-// Four waves of 32 rows each share the tiles of keys and values.  grid (slots * kv_heads): the key heads side by side, so that a
-// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.  Long tiles of a sequence first.
+// 128 query rows of a key head, as one of four waves sees them.
+struct SeqTile {
+  SeqSpan sp;
+  SeqKeys x;
+  int b, head, rows, w0, row, token, h, place, w_first, w_last, t_lo, t_hi;  // tiles of keys [t_lo, t_hi)
+};
+template <int BM, int BN, bool PAGED>
+__device__ __forceinline__ bool seq_tile(const SeqArgs& a, int slot, int head, SeqTile& s, int wave, int lane) {
+  s.b = __builtin_amdgcn_readfirstlane(seq_of_slot(a, slot, BM, lane));
+  s.head = head;
+  s.sp = seq_span(a, s.b);
+  s.rows = s.sp.n * a.group;
+  if (PAGED && s.rows <= 32) return false;  // k_seq_rows
+  // long tiles of a sequence first
+  const int tiles = (s.rows + BM - 1) / BM, tile = tiles - 1 - (slot - seq_slot_base(a, s.b, BM));
+  if (tile < 0 || tile >= tiles) return false;
+  auto place_of = [&](int r) __attribute__((always_inline)) { return s.sp.length - s.sp.n + (r < s.rows ? r : s.rows - 1) / a.group; };
+  const int r0 = tile * BM;
+  s.w0 = r0 + 32 * wave;
+  s.row = s.w0 + (lane & 31);
+  s.x = seq_keys(a, s.b, head, s.sp, place_of(r0), place_of(r0 + BM - 1));
+  s.w_first = place_of(s.w0);
+  s.w_last = place_of(s.w0 + 31);
+  s.place = place_of(s.row);
+  const int r = s.row < s.rows ? s.row : s.rows - 1;
+  s.token = r / a.group;
+  s.h = head * a.group + r - s.token * a.group;
+  s.t_lo = s.x.lo / BN;
+  s.t_hi = (s.x.hi + BN - 1) / BN;
+  return true;
+}
+// Tiles [t0, t1) of keys, shared by the four waves, into the state.  tab, bad: of pages (LDS).
 template <class T, int DP, bool PAGED>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqArgs a) {
+__device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s, SeqState<T, DP>& st, int t0, int t1, unsigned lds0, int* tab, int* bad,
+                                             int wave, int lane) {
   typedef SeqTiles<T, DP> S;
   typedef SeqCfg<T, DP> C;
-  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = (int)blockIdx.x % a.kv_heads, slot = (int)blockIdx.x / a.kv_heads;
-  const int b = __builtin_amdgcn_readfirstlane(seq_of_slot(a, slot, S::BM, lane));
-  const SeqSpan sp = seq_span(a, b);
-  const int rows = sp.n * a.group;
-  if (PAGED && rows <= 32) return;  // k_seq_rows
-  const int tiles = (rows + S::BM - 1) / S::BM, tile = tiles - 1 - (slot - seq_slot_base(a, b, S::BM));
-  if (tile < 0 || tile >= tiles) return;
-  auto place_of = [&](int r) __attribute__((always_inline)) { return sp.length - sp.n + (r < rows ? r : rows - 1) / a.group; };
-  const int r0 = tile * S::BM, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
-  SeqKeys x = seq_keys(a, b, head, sp, place_of(r0), place_of(r0 + S::BM - 1));
-  const int w_first = place_of(w0), w_last = place_of(w0 + 31), place = place_of(row);
-  const int token = (row < rows ? row : rows - 1) / a.group, h = head * a.group + (row < rows ? row : rows - 1) - token * a.group;
-  SeqState<T, DP> st;
-  st.load_q(a.q + (sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
-  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
-  const int t_lo = x.lo / S::BN, t_hi = (x.hi + S::BN - 1) / S::BN;
-  auto issue = [&](int t) __attribute__((always_inline)) {
-    const unsigned at = lds0 + (unsigned)((t & 1) * 2 * S::TB);
-    seq_stage<T, DP, S::BN, S::W, PAGED>(a, x, t * S::BN, at, at + S::TB, wave, lane);
-  };
-  char* out = a.out + (sp.first + token) * a.o_token + h * a.o_head;
-  st.clear();
-  if (t_lo < t_hi) issue(t_lo);
-  for (int t = t_lo; t < t_hi; ++t) {
-    wait_vm<0>();     // this tile has landed
-    __syncthreads();  // for every wave, and everyone is done with the tile before
-    if (t + 1 < t_hi) issue(t + 1);
-    const int k0 = t * S::BN;
-    if (k0 > w_last || (a.window > 0 && k0 + S::BN - 1 <= w_first - a.window)) continue;  // nothing that this wave sees
-    const unsigned K = lds0 + (unsigned)((t & 1) * 2 * S::TB), V = K + S::TB;
-    f32x16 s[S::BN / 32];
+  constexpr int NL = S::BN * C::CB / (64 * S::W);
+  static_assert(NL * 64 * S::W == S::BN * C::CB, "whole requests");
+  t0 = __builtin_amdgcn_readfirstlane(t0);
+  t1 = __builtin_amdgcn_readfirstlane(t1);
+  const int half = lane >> 5, most = PAGED ? seq_table_steps(a.kv, S::BN) : t1 - t0;
+  for (int c0 = t0; c0 < t1; c0 += most) {
+    const int c1 = t1 - c0 < most ? t1 : c0 + most;
+    const int ka = c0 * S::BN > s.x.lo ? c0 * S::BN : s.x.lo, kb = c1 * S::BN < s.x.hi ? c1 * S::BN : s.x.hi;
+    int p0 = 0;
+    if constexpr (PAGED) {
+      __syncthreads();
+      p0 = seq_table(a.kv, s.x.table, ka, kb, tab, bad);
+      __syncthreads();
+    }
+    auto issue = [&](int t) __attribute__((always_inline)) {
+      const unsigned K = lds0 + (unsigned)((t & 1) * 2 * S::TB), V = K + S::TB;
 #pragma unroll
-    for (int n = 0; n < S::BN / 32; ++n) s[n] = st.scores(K, 32 * n, lane);
-    if (k0 + S::BN - 1 > w_first || (a.window > 0 && k0 <= w_last - a.window)) {
+      for (int j = 0; j < NL; ++j) {
+        const int i = (S::W * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+        int place = t * S::BN + r;
+        place = place < ka ? ka : (place >= kb ? kb - 1 : place);
+        int64_t ko, vo;
+        if constexpr (PAGED) {
+          const int p = seq_page(a.kv, place), slot = place - p * a.kv.page_size, page = tab[p - p0];
+          ko = page * a.kv.k_page + slot * a.kv.k_slot;
+          vo = page * a.kv.v_page + slot * a.kv.v_slot;
+        } else {
+          ko = place * a.kv.k_slot;
+          vo = place * a.kv.v_slot;
+        }
+        const unsigned at = (unsigned)((S::W * j + wave) * 1024);
+        dma_x4_from(c < a.kchunks ? s.x.k + ko + 16 * c : (const char*)&seq_zeros, K + at);
+        dma_x4_from(c < a.vchunks ? s.x.v + vo + 16 * c : (const char*)&seq_zeros, V + at);
+        if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    issue(c0);
+    for (int t = c0; t < c1; ++t) {
+      wait_vm<0>();     // this tile has landed
+      __syncthreads();  // for every wave, and everyone is done with the tile before
+      if (t + 1 < c1) issue(t + 1);
+      const int k0 = t * S::BN;
+      if (k0 > s.w_last || (a.window > 0 && k0 + S::BN - 1 <= s.w_first - a.window)) continue;  // nothing that this wave sees
+      const unsigned K = lds0 + (unsigned)((t & 1) * 2 * S::TB), V = K + S::TB;
+      f32x16 p[S::BN / 32];
+#pragma unroll
+      for (int n = 0; n < S::BN / 32; ++n) p[n] = st.scores(K, 32 * n, lane);
+      if (k0 + S::BN - 1 > s.w_first || (a.window > 0 && k0 <= s.w_last - a.window)) {
+#pragma unroll
+        for (int n = 0; n < S::BN / 32; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int back = s.place - (k0 + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3));
+            if (back < 0 || (a.window > 0 && back >= a.window)) p[n][i] = -INFINITY;
+          }
+      }
+      float mx = -INFINITY;
 #pragma unroll
       for (int n = 0; n < S::BN / 32; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int back = place - (k0 + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3));
-          if (back < 0 || (a.window > 0 && back >= a.window)) s[n][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, p[n][i]);
+      st.follow(xor32_max(mx), a.c);
+#pragma unroll
+      for (int n = 0; n < S::BN / 32; ++n) st.add(st.weigh(p[n], a.c), V, 32 * n, lane);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < S::BN / 32; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
-    st.follow(xor32_max(mx), a.c);
-#pragma unroll
-    for (int n = 0; n < S::BN / 32; ++n) st.add(st.weigh(s[n], a.c), V, 32 * n, lane);
   }
-  const bool bad = PAGED && __syncthreads_or(x.bad);
-  const float l = xor32_sum(st.l), f = bad ? NAN : (l == 0.f ? 0.f : 1.0f / l);
-  if (row < rows) {
+}
+// The wave's 32 rows, l being those of both halves; rows with what is no number once more, with care.
+template <class T, int DP, bool PAGED>
+__device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, const SeqState<T, DP>& st, float l, bool bad, int lane) {
+  typedef SeqCfg<T, DP> C;
+  const float f = bad ? NAN : (l == 0.f ? 0.f : 1.0f / l);
+  if (s.row < s.rows) {
+    char* out = a.out + (s.sp.first + s.token) * a.o_token + s.h * a.o_head;
 #pragma unroll
     for (int n = 0; n < C::NMB; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int d = 32 * n + 8 * g + 4 * half;
+        const int d = 32 * n + 8 * g + 4 * (lane >> 5);
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = st.o[n][4 * g + i] * f;
         if (d < a.vchunks * C::E) *(typename Tile<T>::quad*)(out + d * (int)sizeof(T)) = to_quad<T>(v);
       }
   }
-  if (!bad && __builtin_amdgcn_ballot_w64(st.odd())) {
+  if (__builtin_amdgcn_ballot_w64(!bad && st.odd())) {
     wait_vm<0>();  // what is above is written
-    for (int r = w0; r < w0 + 32 && r < rows; ++r) {
-      const int tk = r / a.group, hd = head * a.group + r - tk * a.group;
-      seq_one<T, PAGED>(a, x, a.q + (sp.first + tk) * a.q_token + hd * a.q_head, a.out + (sp.first + tk) * a.o_token + hd * a.o_head,
-                        place_of(r), lane);
+    s.x.bad = false;
+    for (int r = s.w0; r < s.w0 + 32 && r < s.rows; ++r) {
+      const int tk = r / a.group, hd = s.head * a.group + r - tk * a.group;
+      seq_one<T, PAGED>(a, s.x, a.q + (s.sp.first + tk) * a.q_token + hd * a.q_head, a.out + (s.sp.first + tk) * a.o_token + hd * a.o_head,
+                        s.sp.length - s.sp.n + tk, lane);
     }
   }
+}
+
+// Four waves of 32 rows each share the tiles of keys and values.  grid (slots * kv_heads): the key heads side by side, so that a
+// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.
+template <class T, int DP, bool PAGED>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqArgs a) {
+  typedef SeqTiles<T, DP> S;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  int *tab = (int*)(smem_raw + S::RING), *bad = tab + SEQ_TAB;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = (int)blockIdx.x % a.kv_heads, slot = (int)blockIdx.x / a.kv_heads;
+  SeqTile s;
+  if (!seq_tile<S::BM, S::BN, PAGED>(a, slot, head, s, wave, lane)) return;
+  if (PAGED && threadIdx.x == 0) *bad = s.x.bad;
+  SeqState<T, DP> st;
+  st.load_q(a.q + (s.sp.first + s.token) * a.q_token + s.h * a.q_head, lane >> 5, a.kchunks);
+  st.clear();
+  seq_tile_run<T, DP, PAGED>(a, s, st, s.t_lo, s.t_hi, (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw)), tab, bad, wave, lane);
+  if (PAGED) __syncthreads();
+  seq_tile_write<T, DP, PAGED>(a, s, st, xor32_sum(st.l), PAGED && *bad, lane);
 }
 
 // ---- few rows a sequence ---------------------------------------------------------------------------------------------------------
@@ -469,7 +547,6 @@ struct SeqUnits {
   int rows, blocks, lo, hi, t0, steps;  // of each of blocks * kv_heads units
 };
 constexpr int SEQ_STEP = 128;     // four waves of 32 keys
-constexpr int SEQ_SHARES = 512;   // the most: two workgroups on each of MI355X's 256 CUs
 __device__ __forceinline__ SeqUnits seq_units(const SeqRowsArgs& a, int b) {
   SeqUnits u;
   u.sp = seq_span(a.s, b);
@@ -515,7 +592,10 @@ __device__ __forceinline__ SeqScan seq_scan(const SeqRowsArgs& a, int64_t* red /
   return r;
 }
 // Of N workgroups, those that have work, and where the share of one begins.
-__device__ __forceinline__ int seq_shares(int64_t total, int n) { return total < n ? (int)total : n; }
+__device__ __forceinline__ int seq_shares(int64_t total, int n, int least = 1) {
+  const int64_t m = (total + least - 1) / least;
+  return m < n ? (int)m : n;
+}
 __device__ __forceinline__ int64_t seq_share(int64_t total, int n, int i) { return total * i / n; }
 __device__ __forceinline__ int seq_owner(int64_t total, int n, int64_t step) { return (int)(((step + 1) * n - 1) / total); }
 
@@ -528,9 +608,8 @@ struct SeqRows {
   static constexpr int NL = 32 * C::CB / 64;  // requests for one
   static constexpr int PITCH = DP + 1;        // of a row of partial outputs, in the same place
   static constexpr int RING = 4 * NB * TB > 16 * 32 * PITCH ? 4 * NB * TB : 16 * 32 * PITCH;
-  static constexpr int TAB = 1024;  // pages looked up at once
-  static constexpr int LDS = RING + 4 * TAB + 1024 + 64;
-  static_assert(32 * SEQ_SHARES * 4 <= RING && 4096 <= 4 * TAB, "the parts' weights fit the ring, their sums the table");
+  static constexpr int LDS = RING + 4 * SEQ_TAB + 1024 + 64;
+  static_assert(32 * SEQ_SHARES * 4 <= RING && 4096 <= 4 * SEQ_TAB, "the parts' weights fit the ring, their sums the table");
   static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
 };
 
@@ -620,7 +699,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
   typedef SeqCfg<T, DP> C;
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   int* tab = (int*)(smem_raw + S::RING);
-  float *ms = (float*)(tab + S::TAB), *ls = ms + 128;
+  float *ms = (float*)(tab + SEQ_TAB), *ls = ms + 128;
   int64_t* red = (int64_t*)(ls + 128);
   int* flag = (int*)(red + 4);
   const SeqArgs& a = ra.s;
@@ -667,20 +746,12 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
     st.load_q(a.q + (u.sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
     st.clear();
     if (threadIdx.x == 0) flag[1] = x.bad;
-    const int per_table = (S::TAB - 1) * (int64_t)a.kv.page_size / SEQ_STEP < 1 << 20 ? (int)((S::TAB - 1) * (int64_t)a.kv.page_size / SEQ_STEP) : 1 << 20;
+    const int per_table = seq_table_steps(a.kv, SEQ_STEP);
     for (int c0 = ta; c0 < tb && u.hi > u.lo; c0 += per_table) {
       const int c1 = tb - c0 < per_table ? tb : c0 + per_table;
-      // pages of these steps
       const int ka = (u.t0 + c0) * SEQ_STEP > u.lo ? (u.t0 + c0) * SEQ_STEP : u.lo, kb = (u.t0 + c1) * SEQ_STEP < u.hi ? (u.t0 + c1) * SEQ_STEP : u.hi;
-      auto page_of = [&](int k) __attribute__((always_inline)) { return a.kv.magic ? (int)(__umulhi((uint32_t)k, a.kv.magic) >> a.kv.shift) : k; };
-      const int p0 = page_of(ka), np = page_of(kb - 1) - p0 + 1;
       __syncthreads();  // the table before, and partial outputs, are read
-      for (int i = threadIdx.x; i < np; i += 256) {
-        const int page = x.table[p0 + i];
-        const bool ok = (unsigned)page < (unsigned)a.kv.n_pages;
-        tab[i] = ok ? page : 0;
-        if (!ok) flag[1] = 1;
-      }
+      const int p0 = seq_table(a.kv, x.table, ka, kb, tab, flag + 1);
       __syncthreads();
       // half h of these steps: the keys (h even) or the values of step h / 2
       const int halves = 2 * (c1 - c0);
@@ -696,7 +767,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
           const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
           int key = k0 + r;
           key = key < ka ? ka : (key >= kb ? kb - 1 : key);
-          const int p = page_of(key), sl = key - p * a.kv.page_size, page = tab[p - p0];
+          const int p = seq_page(a.kv, key), sl = key - p * a.kv.page_size, page = tab[p - p0];
           dma_x4_from(c < chunks ? base + page * ps + sl * ss + 16 * c : (const char*)&seq_zeros, dst + 1024 * j);
           if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
@@ -802,7 +873,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
         if (flag[0]) __hip_atomic_store(&ra.brought[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
-      if (!flag[0]) continue;
+      if (!__builtin_amdgcn_readfirstlane(flag[0])) continue;
       odd = seq_join<T>(ra, u, head, r0, n_rows, i0, parts, (float*)smem_raw, ls, (f32x4*)tab, wave, lane);
     }
     odd = __syncthreads_or(odd);
@@ -810,4 +881,149 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
   }
 }
 
+
+// ---- many rows, few tiles ----------------------------------------------------------------------------------------------------------
+// Tiles of 128 rows over long keys that are too few for the chip - a portion of a prompt behind a long context - are dealt like the
+// units above: key head after key head, a head's tiles one behind the other, each as many steps as it has tiles of keys.  A part lies in the
+// workspace as it lay in the registers ([wave][o ..., m, l][lane]), so that the workgroup that adds the parts reads it lane by lane.
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_shares(const SeqRowsArgs ra, int slots) {
+  typedef SeqTiles<T, DP> S;
+  typedef SeqCfg<T, DP> C;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  int *tab = (int*)(smem_raw + S::RING), *flag = tab + SEQ_TAB, *red = flag + 4, *pre = flag + 16;  // pre[i]: steps of a head ahead of slot i
+  const SeqArgs& a = ra.s;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
+  // ---- steps of every slot
+  for (int i = threadIdx.x; i <= a.n_seqs && i < SEQ_TAB; i += 256) tab[i] = a.offsets[i];
+  __syncthreads();
+  auto base_of = [&](int b) __attribute__((always_inline)) {
+    const int o = b < SEQ_TAB ? tab[b] : a.offsets[b];
+    return (int)((int64_t)(o < 0 ? 0 : (o > a.n_tokens ? a.n_tokens : o)) * a.group / S::BM) + b;
+  };
+  const int per = (slots + 255) / 256, first = (int)threadIdx.x * per;
+  int mine = 0;
+  for (int i = first; i < first + per && i < slots; ++i) {
+    int lo = 0, n = a.n_seqs;  // the last sequence whose base is at most i
+    while (n > 1) {
+      const int m = n / 2;
+      if (base_of(lo + m) <= i) {
+        lo += m;
+        n -= m;
+      } else {
+        n = m;
+      }
+    }
+    const SeqSpan sp = seq_span(a, lo);
+    const int rows = sp.n * a.group, tiles = (rows + S::BM - 1) / S::BM, tile = tiles - 1 - (i - base_of(lo));
+    int steps = 0;
+    if (rows > 32 && tile >= 0 && tile < tiles) {
+      const int r1 = tile * S::BM + S::BM - 1 < rows ? tile * S::BM + S::BM - 1 : rows - 1;
+      const int p0 = sp.length - sp.n + tile * S::BM / a.group, p1 = sp.length - sp.n + r1 / a.group;
+      const int k0 = a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;
+      steps = (p1 + S::BN) / S::BN - k0 / S::BN;
+      if (p1 < 0 || steps < 1) steps = 1;  // no key at all: a step that writes the zeros
+    }
+    pre[i + 1] = mine += steps;
+  }
+  int x = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) red[wave] = x;
+  __syncthreads();
+  x -= mine;
+  for (int w = 0; w < wave; ++w) x += red[w];
+  for (int i = first; i < first + per && i < slots; ++i) pre[i + 1] += x;
+  if (threadIdx.x == 0) pre[0] = 0;
+  __syncthreads();
+  auto ahead = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(pre[i]); };
+  const int each = ahead(slots);
+  const int64_t total = (int64_t)each * a.kv_heads;
+  if (total == 0) return;
+  // ---- this workgroup's share: those of an XCD side by side, as their keys are
+  const int n_shares = seq_shares(total, ra.shares, S::LEAST), side = (n_shares + 7) / 8;
+  const int share = (int)blockIdx.x % 8 * side + (int)blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= side || share >= n_shares) return;
+  int64_t at = seq_share(total, n_shares, share);
+  const int64_t end = seq_share(total, n_shares, share + 1);
+  int slot = 0;
+  {  // the slot of the first step
+    const int r = (int)(at % each);
+    int n = slots;
+    while (n > 1) {
+      const int m = n / 2;
+      if (ahead(slot + m) <= r) {
+        slot += m;
+        n -= m;
+      } else {
+        n = m;
+      }
+    }
+  }
+  int head = (int)(at / each);
+  while (at < end) {
+    while (ahead(slot + 1) == ahead(slot) || (int64_t)head * each + ahead(slot + 1) <= at)
+      if (++slot == slots) {
+        slot = 0;
+        ++head;
+      }
+    const int64_t s0 = (int64_t)head * each + ahead(slot);
+    const int steps = ahead(slot + 1) - ahead(slot), ta = (int)(at - s0), tb = steps - ta < end - at ? steps : ta + (int)(end - at);
+    at += tb - ta;
+    SeqTile s;
+    (void)seq_tile<S::BM, S::BN, true>(a, slot, head, s, wave, lane);
+    if (threadIdx.x == 0) flag[1] = s.x.bad;
+    SeqState<T, DP> st;
+    st.load_q(a.q + (s.sp.first + s.token) * a.q_token + s.h * a.q_head, lane >> 5, a.kchunks);
+    st.clear();
+    const int t1 = s.t_lo + tb < s.t_hi ? s.t_lo + tb : s.t_hi;
+    seq_tile_run<T, DP, true>(a, s, st, s.t_lo + ta, t1, lds0, tab, flag + 1, wave, lane);
+    __syncthreads();
+    float l = flag[1] ? NAN : xor32_sum(st.l);
+    if (ta != 0 || tb != steps) {
+      const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64;  // of a wave
+      const int i0 = seq_owner(total, n_shares, s0), parts = seq_owner(total, n_shares, s0 + steps - 1) - i0 + 1;
+      float* to = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
+#pragma unroll
+      for (int n = 0; n < C::NMB; ++n)
+        if (n < blocks)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) seq_give(to + (16 * n + i) * 64, st.o[n][i]);
+      seq_give(to + (16 * blocks) * 64, st.m);
+      seq_give(to + (16 * blocks + 1) * 64, l);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        flag[0] = __hip_atomic_fetch_add(&ra.brought[i0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        if (flag[0]) __hip_atomic_store(&ra.brought[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (!__builtin_amdgcn_readfirstlane(flag[0])) continue;
+      // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
+      auto part = [&](int p) __attribute__((always_inline)) {
+        return ra.ws + (size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
+      };
+      float m = -INFINITY;
+      for (int p = 0; p < parts; ++p) m = fmaxf(m, seq_take(part(p) + (16 * blocks) * 64));
+      st.clear();
+      l = 0.f;
+      for (int p = 0; p < parts; ++p) {
+        const float* from = part(p);
+        const float mp = seq_take(from + (16 * blocks) * 64), lp = seq_take(from + (16 * blocks + 1) * 64);
+        const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
+        l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
+#pragma unroll
+        for (int n = 0; n < C::NMB; ++n)
+          if (n < blocks)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[n][i] = __builtin_fmaf(seq_take(from + (16 * n + i) * 64), f, st.o[n][i]);
+      }
+    }
+    seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
+  }
+}
 }  // namespace khm

@@ -48,33 +48,38 @@ SeqArgs args_of(const kh_attn_rows* r, int e) {
   return a;
 }
 
-template <class K, class A>
-int launch(K kern, dim3 grid, int threads, int lds, const A& a, hipStream_t s) {
+template <class K, class... A>
+int launch(K kern, dim3 grid, int lds, hipStream_t s, const A&... a) {
   if (lds > 64 * 1024) KH_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL(kern, grid, dim3(threads), lds, s, a);
+  hipLaunchKernelGGL(kern, grid, dim3(256), lds, s, a...);
   return kh_launch_status();
 }
 
-template <class T, int DP, bool PAGED>
-int tiles(const SeqArgs& a, hipStream_t s) {
+template <class T, int DP>
+int tiles(const SeqRowsArgs& a, bool paged, hipStream_t s) {
   typedef SeqTiles<T, DP> S;
-  const int64_t slots = (int64_t)a.n_tokens * a.group / S::BM + a.n_seqs;
-  return launch(k_seq_tiles<T, DP, PAGED>, dim3((unsigned)(slots * a.kv_heads)), 64 * S::W, S::LDS, a, s);
+  const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
+  const dim3 grid((unsigned)(slots * a.s.kv_heads));
+  if (!paged) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
+  if (slots <= S::MOST && slots * a.s.kv_heads <= 4 * S::SHARES) {
+    SeqRowsArgs b = a;
+    b.shares = S::SHARES;
+    return launch(k_seq_shares<T, DP>, dim3(b.shares), S::LDS_SHARES, s, b, (int)slots);
+  }
+  return launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
 }
 
 template <class T, int DP>
 int rows(SeqRowsArgs a, hipStream_t s) {
   a.shares = SeqRows<T, DP>::SHARES;
-  return launch(k_seq_rows<T, DP>, dim3(a.shares), 256, SeqRows<T, DP>::LDS, a, s);
+  return launch(k_seq_rows<T, DP>, dim3(a.shares), SeqRows<T, DP>::LDS, s, a);
 }
 
-template <bool PAGED>
-int go(const SeqArgs& a, int e, hipStream_t s) {
-  const int most = (a.kchunks > a.vchunks ? a.kchunks : a.vchunks) * 16 / e;
-  if (e == 2) return most <= 64 ? tiles<bf16, 64, PAGED>(a, s) : (most <= 128 ? tiles<bf16, 128, PAGED>(a, s) : tiles<bf16, 256, PAGED>(a, s));
-  return most <= 64 ? tiles<float, 64, PAGED>(a, s) : (most <= 128 ? tiles<float, 128, PAGED>(a, s) : tiles<float, 256, PAGED>(a, s));
+int go(const SeqRowsArgs& a, int e, bool paged, hipStream_t s) {
+  const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
+  if (e == 2) return most <= 64 ? tiles<bf16, 64>(a, paged, s) : (most <= 128 ? tiles<bf16, 128>(a, paged, s) : tiles<bf16, 256>(a, paged, s));
+  return most <= 64 ? tiles<float, 64>(a, paged, s) : (most <= 128 ? tiles<float, 128>(a, paged, s) : tiles<float, 256>(a, paged, s));
 }
-
 int go_rows(const SeqRowsArgs& a, int e, hipStream_t s) {
   const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
   if (e == 2) return most <= 64 ? rows<bf16, 64>(a, s) : (most <= 128 ? rows<bf16, 128>(a, s) : rows<bf16, 256>(a, s));
@@ -91,19 +96,23 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
   if (!k || !v || !kh_aligned16(k) || !kh_aligned16(v) || !khm::whole(k_token, e) || !khm::whole(k_head, e) || !khm::whole(v_token, e) ||
       !khm::whole(v_head, e))
     return KH_ERR_INVALID_ARG;
-  khm::SeqArgs a = khm::args_of(r, e);
+  khm::SeqRowsArgs ra{khm::args_of(r, e)};
+  khm::SeqArgs& a = ra.s;
   a.kv.k = (const char*)k;
   a.kv.v = (const char*)v;
   a.kv.k_slot = k_token * e;
   a.kv.k_head = k_head * e;
   a.kv.v_slot = v_token * e;
   a.kv.v_head = v_head * e;
-  return khm::go<false>(a, e, (hipStream_t)stream);
+  return khm::go(ra, e, false, (hipStream_t)stream);
 }
 
 extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
   if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
-  return (int64_t)khm::SEQ_SHARES * 4 + (int64_t)2 * khm::SEQ_SHARES * 32 * (value_size + 4) * 4;
+  // two parts of a share: 32 rows, or 128 as four waves hold them where a call can have as many
+  const bool tiles = (int64_t)n_tokens * (head_num / kv_head_num) > 32;
+  const int64_t few = 32 * (value_size + 4), many = tiles ? (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0;
+  return 4 * (khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * (few > many ? few : many));
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
@@ -120,7 +129,8 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
       !khm::whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
       workspace_bytes < kh_attn_paged_workspace_bytes(r->head_num, r->kv_head_num, r->value_size, r->n_tokens))
     return KH_ERR_INVALID_ARG;
-  khm::SeqArgs a = khm::args_of(r, e);
+  khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + khm::SEQ_SHARES, 0, 0};
+  khm::SeqArgs& a = ra.s;
   a.kv.k = (const char*)c->k;
   a.kv.v = (const char*)c->v;
   a.kv.k_page = c->k_page * e;
@@ -144,9 +154,9 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
   // rows of a sequence: one with more than 32 has tiles of its own
   const int64_t most = (int64_t)(max_new && max_new < r->n_tokens ? max_new : r->n_tokens) * a.group;
   if (most > 32) {
-    const int done = khm::go<true>(a, e, (hipStream_t)stream);
+    const int done = khm::go(ra, e, true, (hipStream_t)stream);
     if (done != KH_OK) return done;
   }
-  khm::SeqRowsArgs ra{a, (int*)workspace, (float*)workspace + khm::SEQ_SHARES, 0, most <= 32};
+  ra.all = most <= 32;
   return khm::go_rows(ra, e, (hipStream_t)stream);
 }

@@ -256,7 +256,9 @@ PAGED = [  # heads, kv_heads, key size, value size, new tokens, lengths, page, w
     (8, 2, 64, 64, [200, 1, 33], [900, 1000, 33], 48, 0), (4, 4, 128, 128, [64], [1000], 128, 0), (12, 1, 64, 64, [1, 3], [333, 77], 1, 0),
     (32, 4, 64, 64, [1, 70, 1], [500, 300, 20], 16, 100), (6, 6, 48, 48, [1, 1], [256, 31], 100, 31), (8, 8, 256, 256, [1, 40], [90, 100], 16, 0),
     (3, 1, 80, 40, [2, 9], [50, 9], 7, 5), (2, 2, 64, 64, [3, 1, 4], [1, 0, 4], 16, 0), (64, 1, 128, 128, [1], [600], 32, 0), (1, 1, 16, 16, [1], [5000], 256, 0),
-    (32, 8, 64, 64, [8, 4], [515, 1027], 64, 0), (16, 1, 192, 128, [1, 2], [300, 100], 64, 0), (32, 8, 64, 64, [1] * 70, list(range(1, 141, 2)), 16, 0)]
+    (32, 8, 64, 64, [8, 4], [515, 1027], 64, 0), (16, 1, 192, 128, [1, 2], [300, 100], 64, 0), (32, 8, 64, 64, [1] * 70, list(range(1, 141, 2)), 16, 0),
+    (128, 128, 16, 16, [2200, 1, 40], [2300, 77, 40], 32, 0), (8, 2, 64, 64, [40] * 9 + [1] * 3, [3000, 40, 41, 2000, 777, 90, 64, 1000, 50, 9, 4000, 1], 16, 700),
+    (8, 1, 64, 64, [130], [2500], 1, 0)]
 
 
 def check_paged(q, out, lens, new, ks, vs, window, what=""):
