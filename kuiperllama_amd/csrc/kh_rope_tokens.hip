@@ -93,9 +93,120 @@ __global__ __launch_bounds__(256) void k_rope_pairs(const RopeArgs<T> a) {
     }
 }
 
+// The same by 16 bytes: a thread has two vectors of a head's row, E pairs in all - the vectors i of the two halves, or neighbours i - and
+// keeps their cosines and sines for every head that it comes to, BATCH rows requested together.  HBM bounds it.  grid (tokens)
+template <class T, bool STORE>
+__global__ __launch_bounds__(256) void k_rope_rows(const RopeArgs<T> a) {
+  typedef typename Tile<T>::frag frag;
+  constexpr int E = Tile<T>::N, BATCH = 4;
+  const int t = blockIdx.x, per = a.dim / (2 * E), lead = (int)threadIdx.x / per, i = (int)threadIdx.x - lead * per, side = 256 / per;
+  const int both = a.heads + a.kv_heads, turned = a.rot / (2 * E);
+  const bool rotates = i < turned;
+  // two vectors of a row, in elements
+  const int c0 = E * (rotates ? (a.half ? i : 2 * i) : 2 * i), c1 = rotates && a.half ? c0 + a.rot / 2 : c0 + E;
+  const int64_t pos = a.positions[t];
+  int page = 0, slot = 0;
+  const bool kept = !STORE || place(a, t, page, slot);
+  auto from = [&](int r) __attribute__((always_inline)) {
+    return r < a.heads ? a.q + t * a.q_token + r * a.q_head : a.k + t * a.k_token + (r - a.heads) * a.k_head;
+  };
+  auto to = [&](int r) __attribute__((always_inline)) {
+    if (r < a.heads) return a.qo + t * a.qo_token + r * a.qo_head;
+    return (STORE ? a.ko + page * a.k_page + slot * a.ko_token : a.ko + t * a.ko_token) + (r - a.heads) * a.ko_head;
+  };
+  frag x[BATCH], y[BATCH];
+  auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = r0 + j * side;
+      if (r < both) {
+        const T* p = from(r);
+        x[j] = *(const frag*)(p + c0);
+        y[j] = *(const frag*)(p + c1);
+      }
+    }
+  };
+  const bool mine = lead < side;
+  if (mine) load(lead);
+  // values, as they are
+  constexpr int VB = 2;
+  frag v[VB];
+  const int vper = STORE ? a.vdim / E : 1, values = STORE && kept ? a.kv_heads * vper : 0;
+  auto vat = [&](int w, int& h) __attribute__((always_inline)) {
+    h = w / vper;
+    return E * (w - h * vper);
+  };
+  int h;
+#pragma unroll
+  for (int j = 0; j < VB; ++j)
+    if ((int)threadIdx.x + 256 * j < values) {
+      const int d = vat((int)threadIdx.x + 256 * j, h);
+      v[j] = *(const frag*)(a.v + t * a.v_token + h * a.v_head + d);
+    }
+  float cs[E], sn[E];
+  if (rotates)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      cos_sin((uint64_t)pos * a.turns[i * E + e], cs[e], sn[e]);
+      cs[e] *= a.magnitude;
+      sn[e] *= a.magnitude;
+    }
+  if (mine)
+    for (int r0 = lead; r0 < both; r0 += BATCH * side) {
+      if (r0 != lead) load(r0);
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int r = r0 + j * side;
+        if (r >= both || (r >= a.heads && !kept)) continue;
+        frag u = x[j], w = y[j];
+        if (rotates) {
+          if (a.half) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float p = (float)x[j][e], q = (float)y[j][e];
+              u[e] = (T)(p * cs[e] - q * sn[e]);
+              w[e] = (T)(p * sn[e] + q * cs[e]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float p = (float)(e < E / 2 ? x[j][2 * e % E] : y[j][2 * e % E]), q = (float)(e < E / 2 ? x[j][(2 * e + 1) % E] : y[j][(2 * e + 1) % E]);
+              const T lo = (T)(p * cs[e] - q * sn[e]), hi = (T)(p * sn[e] + q * cs[e]);
+              if (e < E / 2) {
+                u[2 * e % E] = lo;
+                u[(2 * e + 1) % E] = hi;
+              } else {
+                w[2 * e % E] = lo;
+                w[(2 * e + 1) % E] = hi;
+              }
+            }
+          }
+        }
+        T* p = to(r);
+        *(frag*)(p + c0) = u;
+        *(frag*)(p + c1) = w;
+      }
+    }
+  if (STORE) {
+    T* vo = a.vo + page * a.v_page + slot * a.v_slot;
+#pragma unroll
+    for (int j = 0; j < VB; ++j)
+      if ((int)threadIdx.x + 256 * j < values) {
+        const int d = vat((int)threadIdx.x + 256 * j, h);
+        *(frag*)(vo + h * a.vo_head + d) = v[j];
+      }
+    for (int w = (int)threadIdx.x + 256 * VB; w < values; w += 256) {
+      const int d = vat(w, h);
+      *(frag*)(vo + h * a.vo_head + d) = *(const frag*)(a.v + t * a.v_token + h * a.v_head + d);
+    }
+  }
+}
+
 template <class T, bool STORE>
 int go(const RopeArgs<T>& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_rope_pairs<T, STORE>), dim3(a.tokens), dim3(256), 0, s, a);
+  constexpr int E = Tile<T>::N;
+  if (a.dim % (2 * E) == 0 && a.rot % (2 * E) == 0) hipLaunchKernelGGL((k_rope_rows<T, STORE>), dim3(a.tokens), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_rope_pairs<T, STORE>), dim3(a.tokens), dim3(256), 0, s, a);
   return kh_launch_status();
 }
 

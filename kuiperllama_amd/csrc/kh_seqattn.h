@@ -93,10 +93,11 @@ struct SeqCfg {
   static constexpr int NMB = DP / 32;             // 32-column blocks of the output
   static constexpr bool TIGHT = RB > 256;         // queries and outputs fill the registers: reads of LDS stay near their use
   static constexpr bool HOLD = RB <= 512;         // queries in registers; else read again for each tile, under 128 products of 64 cycles
-  // LDS: chunk c of row r lies in slot c ^ turn(r).  Reads of a column of chunks over rows (keys), and of 32 bytes of four and
-  // four rows (values), then touch every bank once.  turn(r + 8) = turn(r), and turn(4 + i) = turn(4) ^ turn(i): a lane's addresses of a
-  // tile are one of its own, turned by constants.
-  static __device__ __forceinline__ int turn(int r) { return RB == 128 ? ((r >> 1) & 3) * 2 : (r & 7) * 2; }
+  // LDS: chunk c of row r of the keys lies in slot c ^ turn_k(r), of the values in c ^ turn_v(r).  Reads of 16 bytes of 16 rows
+  // (keys), of 32 bytes of four rows (values) then touch every bank once.  turn_v(r + 8) = turn_v(r), turn_v(4 + i) = turn_v(4) ^ turn_v(i),
+  // turn_k(r + 16) = turn_k(r): a lane's addresses of a tile are one of its own, turned by constants.
+  static __device__ __forceinline__ int turn_k(int r) { return RB == 128 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int turn_v(int r) { return RB == 128 ? ((r >> 1) & 3) * 2 : (r & 7) * 2; }
 };
 
 template <class X>
@@ -152,7 +153,7 @@ struct SeqState {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
     const int r = lane & 31;
-    const unsigned at = K + (unsigned)(r * C::RB + 16 * ((lane >> 5) ^ C::turn(r)));
+    const unsigned at = K + (unsigned)(r * C::RB + 16 * ((lane >> 5) ^ C::turn_k(r)));
 #pragma unroll
     for (int b = 0; b < C::NKB; ++b) {
       s = Tile32<T>::mma(lds_read<frag>((at ^ (32 * b)) + r0 * C::RB), C::HOLD ? q[C::HOLD ? b : 0] : query(b, lane >> 5), s);
@@ -188,7 +189,7 @@ struct SeqState {
     const int half = lane >> 5;
     if constexpr (sizeof(T) == 2) {
       const int r = 4 * half + ((lane >> 2) & 3);  // of eight
-      const unsigned at = V + (unsigned)(r * C::RB + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ C::turn(r)) + 8 * (lane & 1));
+      const unsigned at = V + (unsigned)(r * C::RB + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ C::turn_v(r)) + 8 * (lane & 1));
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         bf16x8 b;
@@ -208,12 +209,12 @@ struct SeqState {
         }
       }
     } else {
-      const unsigned at = V + (unsigned)(4 * half * C::RB + 16 * (((lane & 31) >> 2) ^ C::turn(4 * half)) + 4 * (lane & 3));
+      const unsigned at = V + (unsigned)(4 * half * C::RB + 16 * (((lane & 31) >> 2) ^ C::turn_v(4 * half)) + 4 * (lane & 3));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
 #pragma unroll
         for (int n = 0; n < C::NMB; ++n)
-          o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(lds_read<float>((at ^ (16 * C::turn(i & 3) + 128 * n)) + (r0 + 8 * (i >> 2) + (i & 3)) * C::RB), p[i], o[n],
+          o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(lds_read<float>((at ^ (16 * C::turn_v(i & 3) + 128 * n)) + (r0 + 8 * (i >> 2) + (i & 3)) * C::RB), p[i], o[n],
                                                       0, 0, 0);
         if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
@@ -429,7 +430,7 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
       const unsigned K = lds0 + (unsigned)((t & 1) * 2 * S::TB), V = K + S::TB;
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
-        const int i = (S::W * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+        const int i = (S::W * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = i - r * C::CB, ck = c ^ C::turn_k(r), cv = c ^ C::turn_v(r);
         int place = t * S::BN + r;
         place = place < ka ? ka : (place >= kb ? kb - 1 : place);
         int64_t ko, vo;
@@ -442,8 +443,8 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
           vo = place * a.kv.v_slot;
         }
         const unsigned at = (unsigned)((S::W * j + wave) * 1024);
-        dma_x4_from(c < a.kchunks ? s.x.k + ko + 16 * c : (const char*)&seq_zeros, K + at);
-        dma_x4_from(c < a.vchunks ? s.x.v + vo + 16 * c : (const char*)&seq_zeros, V + at);
+        dma_x4_from(ck < a.kchunks ? s.x.k + ko + 16 * ck : (const char*)&seq_zeros, K + at);
+        dma_x4_from(cv < a.vchunks ? s.x.v + vo + 16 * cv : (const char*)&seq_zeros, V + at);
         if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -764,7 +765,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
         const int chunks = keys ? a.kchunks : a.vchunks;
 #pragma unroll
         for (int j = 0; j < S::NL; ++j) {
-          const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ C::turn(r);
+          const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ (keys ? C::turn_k(r) : C::turn_v(r));
           int key = k0 + r;
           key = key < ka ? ka : (key >= kb ? kb - 1 : key);
           const int p = seq_page(a.kv, key), sl = key - p * a.kv.page_size, page = tab[p - p0];
