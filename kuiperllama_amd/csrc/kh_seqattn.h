@@ -371,8 +371,10 @@ struct SeqTiles {
   static constexpr int RING = 4 * TB;                // two tiles of keys and values each
   static constexpr int MOST = 1024;                  // slots whose steps are dealt
   static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
-  static constexpr int SHARES = LDS_SHARES <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
-  static constexpr int LEAST = 512 / BN;             // steps of a share
+#ifndef X_LT
+#define X_LT 512
+#endif
+  static constexpr int LEAST = X_LT / BN;             // steps of a share
 };
 
 // 128 query rows of a key head, as one of four waves sees them.
@@ -612,6 +614,10 @@ struct SeqRows {
   static constexpr int LDS = RING + 4 * SEQ_TAB + 1024 + 64;
   static_assert(32 * SEQ_SHARES * 4 <= RING && 4096 <= 4 * SEQ_TAB, "the parts' weights fit the ring, their sums the table");
   static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
+#ifndef X_LR
+#define X_LR 1
+#endif
+  static constexpr int LEAST = X_LR;  // steps of a share
 };
 
 // The final rows of a unit: o / l, and with care where that is no number.
@@ -694,11 +700,11 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
   return odd;
 }
 
+// Workgroup `share` of k_seq_rows
 template <class T, int DP>
-__global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs ra) {
+__device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char* smem_raw) {
   typedef SeqRows<T, DP> S;
   typedef SeqCfg<T, DP> C;
-  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   int* tab = (int*)(smem_raw + S::RING);
   float *ms = (float*)(tab + SEQ_TAB), *ls = ms + 128;
   int64_t* red = (int64_t*)(ls + 128);
@@ -709,7 +715,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
   const unsigned ring = lds0 + (unsigned)(wave * S::NB * S::TB);
   // ---- this workgroup's share
   const SeqScan sc = seq_scan(ra, red);
-  const int n_shares = seq_shares(sc.total, ra.shares), share = blockIdx.x;
+  const int n_shares = seq_shares(sc.total, ra.shares, S::LEAST);
   if (share >= n_shares) return;
   int64_t at = seq_share(sc.total, n_shares, share);
   const int64_t end = seq_share(sc.total, n_shares, share + 1);
@@ -729,6 +735,7 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
   int b = __builtin_amdgcn_readfirstlane(flag[0]);
   int64_t ahead = *(int64_t*)(flag + 2);  // steps ahead of sequence b
   SeqUnits u = seq_units(ra, b);
+  int p0 = 0, tab_b = -1, tab_ka = 0, tab_kb = 0;  // the table holds the pages of keys [tab_ka, tab_kb) of tab_b, from page p0 on
   while (at < end) {
     while (at >= ahead + (int64_t)u.blocks * a.kv_heads * u.steps) {
       ahead += (int64_t)u.blocks * a.kv_heads * u.steps;
@@ -746,14 +753,19 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
     SeqState<T, DP> st;
     st.load_q(a.q + (u.sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
     st.clear();
-    if (threadIdx.x == 0) flag[1] = x.bad;
+    if (threadIdx.x == 0 && b != tab_b) flag[1] = x.bad;  // and stays set for the sequence: nothing of it is a number then
     const int per_table = seq_table_steps(a.kv, SEQ_STEP);
     for (int c0 = ta; c0 < tb && u.hi > u.lo; c0 += per_table) {
       const int c1 = tb - c0 < per_table ? tb : c0 + per_table;
       const int ka = (u.t0 + c0) * SEQ_STEP > u.lo ? (u.t0 + c0) * SEQ_STEP : u.lo, kb = (u.t0 + c1) * SEQ_STEP < u.hi ? (u.t0 + c1) * SEQ_STEP : u.hi;
       __syncthreads();  // the table before, and partial outputs, are read
-      const int p0 = seq_table(a.kv, x.table, ka, kb, tab, flag + 1);
-      __syncthreads();
+      if (b != tab_b || ka != tab_ka || kb > tab_kb) {  // not that of the key head before
+        p0 = seq_table(a.kv, x.table, ka, kb, tab, flag + 1);
+        tab_b = b;
+        tab_ka = ka;
+        tab_kb = kb;
+        __syncthreads();
+      }
       // half h of these steps: the keys (h even) or the values of step h / 2
       const int halves = 2 * (c1 - c0);
       auto issue = [&](int h) __attribute__((always_inline)) {
@@ -883,15 +895,20 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
 }
 
 
+template <class T, int DP>
+__global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  seq_rows<T, DP>(a, blockIdx.x, smem_raw);
+}
+
 // ---- many rows, few tiles ----------------------------------------------------------------------------------------------------------
 // Tiles of 128 rows over long keys that are too few for the chip - a portion of a prompt behind a long context - are dealt like the
 // units above: key head after key head, a head's tiles one behind the other, each as many steps as it has tiles of keys.  A part lies in the
 // workspace as it lay in the registers ([wave][o ..., m, l][lane]), so that the workgroup that adds the parts reads it lane by lane.
 template <class T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_shares(const SeqRowsArgs ra, int slots) {
+__device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots, int block, char* smem_raw) {
   typedef SeqTiles<T, DP> S;
   typedef SeqCfg<T, DP> C;
-  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   int *tab = (int*)(smem_raw + S::RING), *flag = tab + SEQ_TAB, *red = flag + 4, *pre = flag + 16;  // pre[i]: steps of a head ahead of slot i
   const SeqArgs& a = ra.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -947,8 +964,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_shares(const Seq
   if (total == 0) return;
   // ---- this workgroup's share: those of an XCD side by side, as their keys are
   const int n_shares = seq_shares(total, ra.shares, S::LEAST), side = (n_shares + 7) / 8;
-  const int share = (int)blockIdx.x % 8 * side + (int)blockIdx.x / 8;
-  if ((int)blockIdx.x / 8 >= side || share >= n_shares) return;
+  const int share = block % 8 * side + block / 8;
+  if (block / 8 >= side || share >= n_shares) return;
   int64_t at = seq_share(total, n_shares, share);
   const int64_t end = seq_share(total, n_shares, share + 1);
   int slot = 0;
@@ -1026,5 +1043,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_shares(const Seq
     }
     seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
   }
+}
+
+// Sequences of many rows and of few at once: workgroups for the tiles of the one, behind them those for the keys of the other.
+template <class T, int DP>
+struct SeqMixed {
+  static constexpr int LDS = SeqTiles<T, DP>::LDS_SHARES > SeqRows<T, DP>::LDS ? SeqTiles<T, DP>::LDS_SHARES : SeqRows<T, DP>::LDS;
+  static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;  // of each
+};
+template <class T, int DP>
+__global__ __launch_bounds__(256, (SeqMixed<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_mixed(const SeqRowsArgs tiles, const SeqRowsArgs rows, int slots) {
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  if ((int)blockIdx.x < tiles.shares) seq_tile_shares<T, DP>(tiles, slots, blockIdx.x, smem_raw);
+  else seq_rows<T, DP>(rows, (int)blockIdx.x - tiles.shares, smem_raw);
 }
 }  // namespace khm

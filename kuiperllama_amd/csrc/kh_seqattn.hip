@@ -55,35 +55,35 @@ int launch(K kern, dim3 grid, int lds, hipStream_t s, const A&... a) {
   return kh_launch_status();
 }
 
+// How a call is launched: TILES alone (whole prompts), or over pages - ROWS alone where no sequence has more than 32 of them, else tiles
+// of rows and, at once or behind them, the rows of the sequences that have few.
+enum How { PACKED, FEW, ANY };
 template <class T, int DP>
-int tiles(const SeqRowsArgs& a, bool paged, hipStream_t s) {
+int go(SeqRowsArgs a, How how, hipStream_t s) {
   typedef SeqTiles<T, DP> S;
+  typedef SeqRows<T, DP> R;
+  typedef SeqMixed<T, DP> M;
+  a.shares = R::SHARES;
+  a.all = how == FEW;
+  if (how == FEW) return launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
   const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
   const dim3 grid((unsigned)(slots * a.s.kv_heads));
-  if (!paged) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
-  if (slots <= S::MOST && slots * a.s.kv_heads <= 4 * S::SHARES) {
+  if (how == PACKED) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
+  if (slots <= S::MOST && slots * a.s.kv_heads <= 4 * M::SHARES) {
+    a.shares = M::SHARES;
     SeqRowsArgs b = a;
-    b.shares = S::SHARES;
-    return launch(k_seq_shares<T, DP>, dim3(b.shares), S::LDS_SHARES, s, b, (int)slots);
+    b.brought = a.brought + SEQ_SHARES;
+    b.ws = a.ws + (size_t)2 * SEQ_SHARES * 32 * (a.s.vchunks * (16 / (int)sizeof(T)) + 4);
+    return launch(k_seq_mixed<T, DP>, dim3(2 * M::SHARES), M::LDS, s, b, a, (int)slots);
   }
-  return launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
+  const int rc = launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
+  return rc != KH_OK ? rc : launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
 }
 
-template <class T, int DP>
-int rows(SeqRowsArgs a, hipStream_t s) {
-  a.shares = SeqRows<T, DP>::SHARES;
-  return launch(k_seq_rows<T, DP>, dim3(a.shares), SeqRows<T, DP>::LDS, s, a);
-}
-
-int go(const SeqRowsArgs& a, int e, bool paged, hipStream_t s) {
+int go(const SeqRowsArgs& a, int e, How how, hipStream_t s) {
   const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
-  if (e == 2) return most <= 64 ? tiles<bf16, 64>(a, paged, s) : (most <= 128 ? tiles<bf16, 128>(a, paged, s) : tiles<bf16, 256>(a, paged, s));
-  return most <= 64 ? tiles<float, 64>(a, paged, s) : (most <= 128 ? tiles<float, 128>(a, paged, s) : tiles<float, 256>(a, paged, s));
-}
-int go_rows(const SeqRowsArgs& a, int e, hipStream_t s) {
-  const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
-  if (e == 2) return most <= 64 ? rows<bf16, 64>(a, s) : (most <= 128 ? rows<bf16, 128>(a, s) : rows<bf16, 256>(a, s));
-  return most <= 64 ? rows<float, 64>(a, s) : (most <= 128 ? rows<float, 128>(a, s) : rows<float, 256>(a, s));
+  if (e == 2) return most <= 64 ? go<bf16, 64>(a, how, s) : (most <= 128 ? go<bf16, 128>(a, how, s) : go<bf16, 256>(a, how, s));
+  return most <= 64 ? go<float, 64>(a, how, s) : (most <= 128 ? go<float, 128>(a, how, s) : go<float, 256>(a, how, s));
 }
 }  // namespace
 }  // namespace khm
@@ -104,15 +104,14 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
   a.kv.k_head = k_head * e;
   a.kv.v_slot = v_token * e;
   a.kv.v_head = v_head * e;
-  return khm::go(ra, e, false, (hipStream_t)stream);
+  return khm::go(ra, e, khm::PACKED, (hipStream_t)stream);
 }
 
 extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
   if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
-  // two parts of a share: 32 rows, or 128 as four waves hold them where a call can have as many
+  // counters, and two parts of a share: 32 rows, and 128 as four waves hold them where a call can have as many
   const bool tiles = (int64_t)n_tokens * (head_num / kv_head_num) > 32;
-  const int64_t few = 32 * (value_size + 4), many = tiles ? (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0;
-  return 4 * (khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * (few > many ? few : many));
+  return 4 * (2 * khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * (32 * ((int64_t)value_size + 4) + (tiles ? (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0)));
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
@@ -129,7 +128,7 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
       !khm::whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
       workspace_bytes < kh_attn_paged_workspace_bytes(r->head_num, r->kv_head_num, r->value_size, r->n_tokens))
     return KH_ERR_INVALID_ARG;
-  khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + khm::SEQ_SHARES, 0, 0};
+  khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + 2 * khm::SEQ_SHARES, 0, 0};
   khm::SeqArgs& a = ra.s;
   a.kv.k = (const char*)c->k;
   a.kv.v = (const char*)c->v;
@@ -151,12 +150,6 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
   a.kv.magic = c->page_size == 1 ? 0 : (uint32_t)((1ull << (31 + bits)) / (uint64_t)c->page_size + 1);
   a.kv.shift = bits - 1;
   a.kv.lengths = lengths;
-  // rows of a sequence: one with more than 32 has tiles of its own
   const int64_t most = (int64_t)(max_new && max_new < r->n_tokens ? max_new : r->n_tokens) * a.group;
-  if (most > 32) {
-    const int done = khm::go(ra, e, true, (hipStream_t)stream);
-    if (done != KH_OK) return done;
-  }
-  ra.all = most <= 32;
-  return khm::go_rows(ra, e, (hipStream_t)stream);
+  return khm::go(ra, e, most <= 32 ? khm::FEW : khm::ANY, (hipStream_t)stream);
 }
