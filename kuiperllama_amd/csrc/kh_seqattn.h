@@ -371,10 +371,7 @@ struct SeqTiles {
   static constexpr int RING = 4 * TB;                // two tiles of keys and values each
   static constexpr int MOST = 1024;                  // slots whose steps are dealt
   static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
-#ifndef X_LT
-#define X_LT 512
-#endif
-  static constexpr int LEAST = X_LT / BN;             // steps of a share
+  static constexpr int LEAST = 512 / BN;             // steps of a share
 };
 
 // 128 query rows of a key head, as one of four waves sees them.
@@ -533,7 +530,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqA
 // ---- few rows a sequence ---------------------------------------------------------------------------------------------------------
 // Sequences of up to 32 query rows (single tokens above all) read their keys once, whatever is done: HBM bounds them, so all keys
 // of all sequences are dealt evenly to the workgroups that fit on the chip at once.  A unit is a key head of a sequence; units lie one
-// behind the other, each a number of steps of 128 keys, and workgroup i takes steps [i W / N, (i + 1) W / N) of the W, the
+// behind the other, each a head and a number of steps of 128 keys, and workgroup i takes places [i W / N, (i + 1) W / N) of the W, the
 // end of one unit and the beginning of the next where they fall so.  What it finds of a unit that others have parts of goes to
 // the workspace, fp32 and with its m and l; the workgroup that is the last to bring a part adds them, in the order of the keys whoever
 // it is.  Every workgroup finds its share from the lengths on the device by one sum over the sequences: no table from the host, and a
@@ -544,12 +541,19 @@ struct SeqRowsArgs {
   int* brought;
   float* ws;        // [2 N][32][value size + 4], o, m, l: of the unit that began before workgroup i's share, of the one that ends behind it
   int shares, all;  // N; all: sequences of more than 32 rows too, 32 at a time
+  // the same for tiles of many rows
+  int* brought_tiles;
+  float* ws_tiles;
 };
 struct SeqUnits {
   SeqSpan sp;
   int rows, blocks, lo, hi, t0, steps;  // of each of blocks * kv_heads units
+  int64_t all;                          // places of all of them
 };
 constexpr int SEQ_STEP = 128;     // four waves of 32 keys
+// Places ahead of a unit's first step, for what a unit costs beside its steps: 256 tokens over 100 - 1885 keys at heads of 64, the short ones
+// first, take 169 us without, 109 with 1, 111 with 2, 121 with 5.
+constexpr int SEQ_HEAD = 1;
 __device__ __forceinline__ SeqUnits seq_units(const SeqRowsArgs& a, int b) {
   SeqUnits u;
   u.sp = seq_span(a.s, b);
@@ -561,6 +565,7 @@ __device__ __forceinline__ SeqUnits seq_units(const SeqRowsArgs& a, int b) {
   u.t0 = u.lo / SEQ_STEP;
   const int n = (u.hi + SEQ_STEP - 1) / SEQ_STEP - u.t0;
   u.steps = n > 1 ? n : 1;  // no key at all: a step that writes the zeros
+  u.all = (int64_t)u.blocks * a.s.kv_heads * (u.steps + SEQ_HEAD);
   return u;
 }
 // Steps ahead of each sequence and in all, for a workgroup of 256.  A thread sums `per` sequences that lie side by side.
@@ -575,7 +580,7 @@ __device__ __forceinline__ SeqScan seq_scan(const SeqRowsArgs& a, int64_t* red /
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = (int)threadIdx.x * r.per;
   for (int b = b0; b < b0 + r.per && b < a.s.n_seqs; ++b) {
     const SeqUnits u = seq_units(a, b);
-    r.mine += (int64_t)u.blocks * a.s.kv_heads * u.steps;
+    r.mine += u.all;
   }
   int64_t x = r.mine;
 #pragma unroll
@@ -600,6 +605,14 @@ __device__ __forceinline__ int seq_shares(int64_t total, int n, int least = 1) {
   return m < n ? (int)m : n;
 }
 __device__ __forceinline__ int64_t seq_share(int64_t total, int n, int i) { return total * i / n; }
+// The workgroup that has the first part of a unit of rows, and the number of its parts, those of the workgroups that follow: one more than the
+// borders behind its head.
+__device__ __forceinline__ int seq_parts(int64_t total, int n, int64_t unit, int places, int& first) {
+  const int64_t y = unit + SEQ_HEAD + 1, z = unit + places - 1;
+  const int a = (int)((y * n + total - 1) / total), b = (int)(((z + 1) * n + total - 1) / total) - 1;
+  first = a - 1;
+  return b < a ? 1 : b - a + 2;
+}
 __device__ __forceinline__ int seq_owner(int64_t total, int n, int64_t step) { return (int)(((step + 1) * n - 1) / total); }
 
 template <class T, int DP>
@@ -612,12 +625,8 @@ struct SeqRows {
   static constexpr int PITCH = DP + 1;        // of a row of partial outputs, in the same place
   static constexpr int RING = 4 * NB * TB > 16 * 32 * PITCH ? 4 * NB * TB : 16 * 32 * PITCH;
   static constexpr int LDS = RING + 4 * SEQ_TAB + 1024 + 64;
-  static_assert(32 * SEQ_SHARES * 4 <= RING && 4096 <= 4 * SEQ_TAB, "the parts' weights fit the ring, their sums the table");
+  static_assert(4 * SEQ_SHARES <= RING && 4096 <= 4 * SEQ_TAB, "a row's weights fit the ring, the sums of parts the table");
   static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
-#ifndef X_LR
-#define X_LR 1
-#endif
-  static constexpr int LEAST = X_LR;  // steps of a share
 };
 
 // The final rows of a unit: o / l, and with care where that is no number.
@@ -635,47 +644,66 @@ __device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, 
 // caches that are not common: with 512 workgroups, a fence for each part costs the launch 15 - 20 us.
 __device__ __forceinline__ void seq_give(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float seq_take(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ f32x4 seq_take4(const float* p) {
+  return f32x4{seq_take(p), seq_take(p + 1), seq_take(p + 2), seq_take(p + 3)};
+}
 
-// The rows of a unit from its parts: their weights (LDS, [32][parts]), then their outputs, four columns a thread and as many parts side by
-// side as there are threads.  True where an output is no number.
+// The rows of a unit from its parts: their weights (LDS, as many rows at a time as fit `room` floats), then their outputs, four columns a
+// thread and as many parts side by side as there are threads.  True where an output is no number.
 template <class T>
 __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& u, int head, int r0, int n_rows, int i0, int parts, float* weight,
-                                         float* ls, f32x4* red, int wave, int lane) {
+                                         int room, float* ls, f32x4* red, int wave, int lane) {
   const SeqArgs& a = ra.s;
   const int cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 4;
   // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
   auto at = [&](int r, int p) __attribute__((always_inline)) { return ra.ws + ((size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 32 + r) * pitch; };
-  for (int r = wave; r < n_rows; r += 4) {
-    float m = -INFINITY, l = 0.f;
-    for (int p = lane; p < parts; p += 64) m = fmaxf(m, seq_take(at(r, p) + cols));
-    m = wave_max(m);
-    for (int p = lane; p < parts; p += 64) {
-      const float mp = seq_take(at(r, p) + cols), lp = seq_take(at(r, p) + cols + 1);
-      const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
-      weight[r * parts + p] = f;
-      l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
-    }
-    l = wave_sum(l);
-    if (lane == 0) ls[r] = l;
-  }
-  __syncthreads();
   int across = 1, down = 1;  // threads of a row: its columns by four; rows at once
   while (across * 4 < cols) across *= 2;
-  while (down < n_rows && down * across < 256) down *= 2;
+  while (down < n_rows && down * across < 256 && 2 * down * parts <= room) down *= 2;
   const int side = 256 / (across * down), x = (int)threadIdx.x & (across - 1), y = (int)threadIdx.x / across & (down - 1),
             z = (int)threadIdx.x / (across * down);
   bool odd = false;
   for (int rb = 0; rb < n_rows; rb += down) {
+    for (int r = rb + wave; r < rb + down && r < n_rows; r += 4) {
+      constexpr int PER = SEQ_SHARES / 64;
+      float mp[PER], lp[PER], m = -INFINITY, l = 0.f;  // all requested together
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        mp[k] = -INFINITY;
+        lp[k] = 0.f;
+        if (lane + 64 * k < parts) {
+          mp[k] = seq_take(at(r, lane + 64 * k) + cols);
+          lp[k] = seq_take(at(r, lane + 64 * k) + cols + 1);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) m = fmaxf(m, mp[k]);
+      m = wave_max(m);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const float f = mp[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp[k] - m) * a.c);
+        if (lane + 64 * k < parts) weight[(r - rb) * parts + lane + 64 * k] = f;
+        l += mp[k] == -INFINITY ? lp[k] : lp[k] * f;  // NaN of a page that is none
+      }
+      l = wave_sum(l);
+      if (lane == 0) ls[r] = l;
+    }
+    __syncthreads();
     const int r = rb + y;
     const bool mine = r < n_rows && 4 * x < cols;
     f32x4 o = f4_zero();
     if (mine) {
-#pragma unroll 4
-      for (int p = z; p < parts; p += side) {
-        const float* v = at(r, p) + 4 * x;
-        const float f = weight[r * parts + p];
+      constexpr int DEEP = 4;  // parts requested together
+      for (int p = z; p < parts; p += DEEP * side) {
+        f32x4 v[DEEP];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(seq_take(v + i), f, o[i]);
+        for (int k = 0; k < DEEP; ++k) v[k] = p + k * side < parts ? seq_take4(at(r, p + k * side) + 4 * x) : f4_zero();
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+          const float f = p + k * side < parts ? weight[y * parts + p + k * side] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(v[k][i], f, o[i]);
+        }
       }
     }
     red[threadIdx.x] = o;
@@ -715,7 +743,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
   const unsigned ring = lds0 + (unsigned)(wave * S::NB * S::TB);
   // ---- this workgroup's share
   const SeqScan sc = seq_scan(ra, red);
-  const int n_shares = seq_shares(sc.total, ra.shares, S::LEAST);
+  const int n_shares = seq_shares(sc.total, ra.shares);
   if (share >= n_shares) return;
   int64_t at = seq_share(sc.total, n_shares, share);
   const int64_t end = seq_share(sc.total, n_shares, share + 1);
@@ -723,8 +751,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
     int64_t p = sc.before;
     int b = (int)threadIdx.x * sc.per;
     for (;; ++b) {
-      const SeqUnits u = seq_units(ra, b);
-      const int64_t n = (int64_t)u.blocks * a.kv_heads * u.steps;
+      const int64_t n = seq_units(ra, b).all;
       if (at < p + n) break;
       p += n;
     }
@@ -733,17 +760,19 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
   }
   __syncthreads();
   int b = __builtin_amdgcn_readfirstlane(flag[0]);
-  int64_t ahead = *(int64_t*)(flag + 2);  // steps ahead of sequence b
+  int64_t ahead = *(int64_t*)(flag + 2);  // places ahead of sequence b
   SeqUnits u = seq_units(ra, b);
   int p0 = 0, tab_b = -1, tab_ka = 0, tab_kb = 0;  // the table holds the pages of keys [tab_ka, tab_kb) of tab_b, from page p0 on
   while (at < end) {
-    while (at >= ahead + (int64_t)u.blocks * a.kv_heads * u.steps) {
-      ahead += (int64_t)u.blocks * a.kv_heads * u.steps;
+    while (at >= ahead + u.all) {
+      ahead += u.all;
       u = seq_units(ra, ++b);
     }
-    const int unit = (int)((at - ahead) / u.steps), ta = (int)((at - ahead) - (int64_t)unit * u.steps);
-    const int tb = u.steps - ta < end - at ? u.steps : ta + (int)(end - at);
-    at += tb - ta;
+    const int places = u.steps + SEQ_HEAD, unit = (int)((at - ahead) / places), from = (int)((at - ahead) - (int64_t)unit * places);
+    const int to = places - from < end - at ? places : from + (int)(end - at);
+    at += to - from;
+    const int ta = from > SEQ_HEAD ? from - SEQ_HEAD : 0, tb = to > SEQ_HEAD ? to - SEQ_HEAD : 0;
+    if (tb <= ta) continue;  // nothing but the unit's head: the workgroup that follows begins it
     const int head = unit / u.blocks, r0 = 32 * (unit - head * u.blocks);
     const int n_rows = u.rows - r0 < 32 ? u.rows - r0 : 32;
     const int row = r0 + ((lane & 31) < n_rows ? (lane & 31) : n_rows - 1);
@@ -840,10 +869,14 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
     const float f = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m - m) * a.c);
     float* part = (float*)smem_raw;
     if ((lane & 31) < n_rows) {
+      float* mine = part + (32 * wave + (seq_fresh<C::TIGHT>(lane) & 31)) * S::PITCH + 4 * half;
 #pragma unroll
       for (int n = 0; n < C::NMB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[(32 * wave + (lane & 31)) * S::PITCH + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3)] = st.o[n][i] * f;
+        for (int i = 0; i < 16; ++i) {
+          mine[32 * n + 8 * (i >> 2) + (i & 3)] = st.o[n][i] * f;
+          if (C::TIGHT && i == 15) __builtin_amdgcn_sched_barrier(0);
+        }
     }
     __syncthreads();
     const bool bad = flag[1] != 0;
@@ -877,8 +910,8 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
       }
     }
     if (!whole) {
-      const int64_t s0 = ahead + (int64_t)unit * u.steps;
-      const int i0 = seq_owner(sc.total, n_shares, s0), parts = seq_owner(sc.total, n_shares, s0 + u.steps - 1) - i0 + 1;
+      int i0;
+      const int parts = seq_parts(sc.total, n_shares, ahead + (int64_t)unit * places, places, i0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -887,9 +920,13 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
       }
       __syncthreads();
       if (!__builtin_amdgcn_readfirstlane(flag[0])) continue;
-      odd = seq_join<T>(ra, u, head, r0, n_rows, i0, parts, (float*)smem_raw, ls, (f32x4*)tab, wave, lane);
+      odd = seq_join<T>(ra, u, head, r0, n_rows, i0, parts, (float*)smem_raw, S::RING / 4, ls, (f32x4*)tab, wave, lane);
+      tab_b = -1;
     }
-    odd = __syncthreads_or(odd);
+    const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (lane == 0) flag[4 + wave] = any;
+    __syncthreads();
+    odd = flag[4] | flag[5] | flag[6] | flag[7];
     seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
   }
 }
@@ -1005,7 +1042,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
     if (ta != 0 || tb != steps) {
       const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64;  // of a wave
       const int i0 = seq_owner(total, n_shares, s0), parts = seq_owner(total, n_shares, s0 + steps - 1) - i0 + 1;
-      float* to = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
+      float* to = ra.ws_tiles + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
 #pragma unroll
       for (int n = 0; n < C::NMB; ++n)
         if (n < blocks)
@@ -1016,14 +1053,14 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
       __syncthreads();
       if (threadIdx.x == 0) {
-        flag[0] = __hip_atomic_fetch_add(&ra.brought[i0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
-        if (flag[0]) __hip_atomic_store(&ra.brought[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        flag[0] = __hip_atomic_fetch_add(&ra.brought_tiles[i0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        if (flag[0]) __hip_atomic_store(&ra.brought_tiles[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
       if (!__builtin_amdgcn_readfirstlane(flag[0])) continue;
       // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
       auto part = [&](int p) __attribute__((always_inline)) {
-        return ra.ws + (size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
+        return ra.ws_tiles + (size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
       };
       float m = -INFINITY;
       for (int p = 0; p < parts; ++p) m = fmaxf(m, seq_take(part(p) + (16 * blocks) * 64));
@@ -1045,16 +1082,22 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   }
 }
 
-// Sequences of many rows and of few at once: workgroups for the tiles of the one, behind them those for the keys of the other.
+// Sequences of many rows and of few at once: workgroups for the tiles of the one, behind them those for the keys of the other.  At heads
+// of 256 each fills the registers, and they are launches of their own.
 template <class T, int DP>
 struct SeqMixed {
   static constexpr int LDS = SeqTiles<T, DP>::LDS_SHARES > SeqRows<T, DP>::LDS ? SeqTiles<T, DP>::LDS_SHARES : SeqRows<T, DP>::LDS;
   static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;  // of each
 };
 template <class T, int DP>
-__global__ __launch_bounds__(256, (SeqMixed<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_mixed(const SeqRowsArgs tiles, const SeqRowsArgs rows, int slots) {
+__global__ __launch_bounds__(256, (SeqMixed<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_mixed(const SeqRowsArgs a, int slots) {
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  if ((int)blockIdx.x < tiles.shares) seq_tile_shares<T, DP>(tiles, slots, blockIdx.x, smem_raw);
-  else seq_rows<T, DP>(rows, (int)blockIdx.x - tiles.shares, smem_raw);
+  if ((int)blockIdx.x < a.shares) seq_tile_shares<T, DP>(a, slots, blockIdx.x, smem_raw);
+  else seq_rows<T, DP>(a, (int)blockIdx.x - a.shares, smem_raw);
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256, 1) void k_seq_tile_shares(const SeqRowsArgs a, int slots) {
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  seq_tile_shares<T, DP>(a, slots, blockIdx.x, smem_raw);
 }
 }  // namespace khm

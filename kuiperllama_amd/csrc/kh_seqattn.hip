@@ -71,12 +71,14 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   if (how == PACKED) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
   if (slots <= S::MOST && slots * a.s.kv_heads <= 4 * M::SHARES) {
     a.shares = M::SHARES;
-    SeqRowsArgs b = a;
-    b.brought = a.brought + SEQ_SHARES;
-    b.ws = a.ws + (size_t)2 * SEQ_SHARES * 32 * (a.s.vchunks * (16 / (int)sizeof(T)) + 4);
-    return launch(k_seq_mixed<T, DP>, dim3(2 * M::SHARES), M::LDS, s, b, a, (int)slots);
+    a.brought_tiles = a.brought + SEQ_SHARES;
+    a.ws_tiles = a.ws + (size_t)2 * SEQ_SHARES * 32 * (a.s.vchunks * (16 / (int)sizeof(T)) + 4);
+    if constexpr (DP <= 128) return launch(k_seq_mixed<T, DP>, dim3(2 * M::SHARES), M::LDS, s, a, (int)slots);
   }
-  const int rc = launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
+  int rc;
+  if (DP > 128 && a.ws_tiles) rc = launch(k_seq_tile_shares<T, 256>, dim3(M::SHARES), S::LDS_SHARES, s, a, (int)slots);
+  else rc = launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
+  a.shares = R::SHARES;
   return rc != KH_OK ? rc : launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
 }
 
@@ -128,7 +130,7 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
       !khm::whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
       workspace_bytes < kh_attn_paged_workspace_bytes(r->head_num, r->kv_head_num, r->value_size, r->n_tokens))
     return KH_ERR_INVALID_ARG;
-  khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + 2 * khm::SEQ_SHARES, 0, 0};
+  khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + 2 * khm::SEQ_SHARES};
   khm::SeqArgs& a = ra.s;
   a.kv.k = (const char*)c->k;
   a.kv.v = (const char*)c->v;
