@@ -219,7 +219,7 @@ int check_rows(const kh_rope_rows* r, bool store) {
       r->rot_dim % 2 || r->rot_dim > r->head_size || !(fabsf(r->magnitude) <= 3.4e38f))
     return KH_ERR_INVALID_ARG;
   const int e = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
-  if (!whole(r->head_size, e) || r->head_size > 256) return KH_ERR_UNSUPPORTED;
+  if (!whole(r->head_size, e) || r->head_size > 256 || r->n_tokens >= 1 << 24) return KH_ERR_UNSUPPORTED;  // a grid has 2^32 threads
   if ((r->rot_dim && !r->turns) || !r->positions || !r->q || !r->k || !r->q_out || (!store && !r->k_out) || !kh_aligned16(r->q) || !kh_aligned16(r->k) ||
       !kh_aligned16(r->q_out) || (!store && !kh_aligned16(r->k_out)) || !whole(r->q_token, e) || !whole(r->q_head, e) || !whole(r->k_token, e) ||
       !whole(r->k_head, e) || !whole(r->qo_token, e) || !whole(r->qo_head, e) || (!store && (!whole(r->ko_token, e) || !whole(r->ko_head, e))))

@@ -51,6 +51,7 @@ struct SeqKv {
   int n_pages, page_size, most;  // most: places of a sequence's row of the table
   uint32_t magic;  // place / page_size = umulhi(place, magic) >> shift; 0: page_size 1
   int shift;
+  int plain;  // a request's rows are whole, in one page and evenly apart
   const int32_t* lengths;
 };
 struct SeqArgs {
@@ -111,6 +112,13 @@ __device__ __forceinline__ int seq_fresh(int x) {
   if (YES) asm volatile("" : "+v"(x));
   return x;
 }
+
+// Numbers that are the same in every lane, where the compiler does not see it
+__device__ __forceinline__ int seq_same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t seq_same64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)seq_same((int)(x >> 32)) << 32 | (uint32_t)seq_same((int)x));
+}
+__device__ __forceinline__ const char* seq_same(const char* p) { return (const char*)seq_same64((int64_t)p); }
 
 // The running state of 32 query rows, a lane's row being l & 31.
 template <class T, int DP>
@@ -369,9 +377,9 @@ struct SeqTiles {
   static constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   static constexpr int TB = BN * SeqCfg<T, DP>::RB;  // bytes of a tile of keys
   static constexpr int RING = 4 * TB;                // two tiles of keys and values each
-  static constexpr int MOST = 1024;                  // slots whose steps are dealt
+  static constexpr int MOST = 512;                   // slots that are looked at to be cut
   static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
-  static constexpr int LEAST = 512 / BN;             // steps of a share
+  static constexpr int LEAST = 512 / BN;             // steps of a part
 };
 
 // 128 query rows of a key head, as one of four waves sees them.
@@ -415,18 +423,40 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
   static_assert(NL * 64 * S::W == S::BN * C::CB, "whole requests");
   t0 = __builtin_amdgcn_readfirstlane(t0);
   t1 = __builtin_amdgcn_readfirstlane(t1);
+  const char *kp = seq_same(s.x.k), *vp = seq_same(s.x.v);
   const int half = lane >> 5, most = PAGED ? seq_table_steps(a.kv, S::BN) : t1 - t0;
   for (int c0 = t0; c0 < t1; c0 += most) {
     const int c1 = t1 - c0 < most ? t1 : c0 + most;
-    const int ka = c0 * S::BN > s.x.lo ? c0 * S::BN : s.x.lo, kb = c1 * S::BN < s.x.hi ? c1 * S::BN : s.x.hi;
+    const int ka = seq_same(c0 * S::BN > s.x.lo ? c0 * S::BN : s.x.lo), kb = seq_same(c1 * S::BN < s.x.hi ? c1 * S::BN : s.x.hi);
     int p0 = 0;
     if constexpr (PAGED) {
       __syncthreads();
-      p0 = seq_table(a.kv, s.x.table, ka, kb, tab, bad);
+      p0 = seq_same(seq_table(a.kv, s.x.table, ka, kb, tab, bad));
       __syncthreads();
     }
     auto issue = [&](int t) __attribute__((always_inline)) {
       const unsigned K = lds0 + (unsigned)((t & 1) * 2 * S::TB), V = K + S::TB;
+      if (a.kv.plain && t * S::BN >= ka && t * S::BN + S::BN <= kb) {  // addresses in the scalar unit: one lane's offset serves every request
+        constexpr int RPR = 64 / C::CB;  // rows of a request
+        const int r = lane / C::CB, c = lane % C::CB;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          const int row = (S::W * j + wave) * RPR, place = t * S::BN + row;
+          const char *k = kp, *v = vp;
+          if constexpr (PAGED) {
+            const int p = seq_page(a.kv, place), page = seq_same(tab[p - p0]), slot = place - p * a.kv.page_size;
+            k += page * a.kv.k_page + slot * a.kv.k_slot;
+            v += page * a.kv.v_page + slot * a.kv.v_slot;
+          } else {
+            k += place * a.kv.k_slot;
+            v += place * a.kv.v_slot;
+          }
+          const unsigned at = (unsigned)((S::W * j + wave) * 1024);
+          dma_x4_keep(k, (unsigned)(r * (int)a.kv.k_slot + 16 * (c ^ C::turn_k(row + r))), K + at);
+          dma_x4_keep(v, (unsigned)(r * (int)a.kv.v_slot + 16 * (c ^ C::turn_v(row + r))), V + at);
+        }
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const int i = (S::W * j + wave) * 64 + seq_fresh<C::TIGHT>(lane), r = i / C::CB, c = i - r * C::CB, ck = c ^ C::turn_k(r), cv = c ^ C::turn_v(r);
@@ -508,9 +538,11 @@ __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, con
 }
 
 // Four waves of 32 rows each share the tiles of keys and values.  grid (slots * kv_heads): the key heads side by side, so that a
-// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.
+// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.  8192 tokens of 32 heads over 8: 320 us at heads of
+// 64 (863 TFLOP/s), 585 at 128 (945), where the chip clocks down to 1.86 GHz and the matrix cores are busy 44 % of its cycles, the vector
+// unit (exponentials, maxima) 53.
 template <class T, int DP, bool PAGED>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_seq_tiles(const SeqArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : (DP <= 128 ? 2 : 1)) void k_seq_tiles(const SeqArgs a) {
   typedef SeqTiles<T, DP> S;
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   int *tab = (int*)(smem_raw + S::RING), *bad = tab + SEQ_TAB;
@@ -600,10 +632,7 @@ __device__ __forceinline__ SeqScan seq_scan(const SeqRowsArgs& a, int64_t* red /
   return r;
 }
 // Of N workgroups, those that have work, and where the share of one begins.
-__device__ __forceinline__ int seq_shares(int64_t total, int n, int least = 1) {
-  const int64_t m = (total + least - 1) / least;
-  return m < n ? (int)m : n;
-}
+__device__ __forceinline__ int seq_shares(int64_t total, int n) { return total < n ? (int)total : n; }
 __device__ __forceinline__ int64_t seq_share(int64_t total, int n, int i) { return total * i / n; }
 // The workgroup that has the first part of a unit of rows, and the number of its parts, those of the workgroups that follow: one more than the
 // borders behind its head.
@@ -613,7 +642,6 @@ __device__ __forceinline__ int seq_parts(int64_t total, int n, int64_t unit, int
   first = a - 1;
   return b < a ? 1 : b - a + 2;
 }
-__device__ __forceinline__ int seq_owner(int64_t total, int n, int64_t step) { return (int)(((step + 1) * n - 1) / total); }
 
 template <class T, int DP>
 struct SeqRows {
@@ -779,6 +807,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
     const int token = row / a.group, h = head * a.group + row - token * a.group, place = u.sp.length - u.sp.n + token;
     const int first_place = u.sp.length - u.sp.n + r0 / a.group, last_place = u.sp.length - u.sp.n + (r0 + n_rows - 1) / a.group;
     SeqKeys x = seq_keys(a, b, head, u.sp, u.sp.length - u.sp.n, u.sp.length - 1);
+    const char *kp = seq_same(x.k), *vp = seq_same(x.v);
     SeqState<T, DP> st;
     st.load_q(a.q + (u.sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
     st.clear();
@@ -798,12 +827,23 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
       // half h of these steps: the keys (h even) or the values of step h / 2
       const int halves = 2 * (c1 - c0);
       auto issue = [&](int h) __attribute__((always_inline)) {
-        const int k0 = (u.t0 + c0 + (h >> 1)) * SEQ_STEP + 32 * wave;
+        const int k0 = seq_same((u.t0 + c0 + (h >> 1)) * SEQ_STEP + 32 * wave);
         const unsigned dst = ring + (unsigned)(h % S::NB * S::TB);
         const bool keys = (h & 1) == 0;
-        const char* base = keys ? x.k : x.v;
+        const char* base = keys ? kp : vp;
         const int64_t ps = keys ? a.kv.k_page : a.kv.v_page, ss = keys ? a.kv.k_slot : a.kv.v_slot;
         const int chunks = keys ? a.kchunks : a.vchunks;
+        if (a.kv.plain && k0 >= ka && k0 + 32 <= kb) {  // addresses in the scalar unit
+          constexpr int RPR = 64 / C::CB;
+          const int r = seq_fresh<C::TIGHT>(lane) / C::CB, c = lane % C::CB;
+#pragma unroll
+          for (int j = 0; j < S::NL; ++j) {
+            const int key = k0 + j * RPR, p = seq_page(a.kv, key), page = seq_same(tab[p - p0]);
+            dma_x4_keep(base + page * ps + (key - p * a.kv.page_size) * ss,
+                        (unsigned)(r * (int)ss + 16 * (c ^ (keys ? C::turn_k(j * RPR + r) : C::turn_v(j * RPR + r)))), dst + 1024 * j);
+          }
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < S::NL; ++j) {
           const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ (keys ? C::turn_k(r) : C::turn_v(r));
@@ -939,27 +979,34 @@ __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) vo
 }
 
 // ---- many rows, few tiles ----------------------------------------------------------------------------------------------------------
-// Tiles of 128 rows over long keys that are too few for the chip - a portion of a prompt behind a long context - are dealt like the
-// units above: key head after key head, a head's tiles one behind the other, each as many steps as it has tiles of keys.  A part lies in the
-// workspace as it lay in the registers ([wave][o ..., m, l][lane]), so that the workgroup that adds the parts reads it lane by lane.
+// Tiles of 128 rows over long keys that are too few for the chip - a portion of a prompt behind a long context - are cut along their
+// keys: every tile into as many equal parts of at most T steps as it takes, with the least T whose parts are no more than the workgroups
+// that fit on the chip at once.  (Dealt like the units above, at borders wherever they fall, a workgroup has two parts to hand over and
+// not one: 64 KB each, 8 x 256 tokens behind 1792 keys 138 us, 91 where no tile is cut.)  A part lies in the workspace as it lay in the
+// registers ([wave][o ..., m, l][lane]), so that the workgroup that adds the parts, the last one to bring one, reads it lane by lane.
 template <class T, int DP>
 __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots, int block, char* smem_raw) {
   typedef SeqTiles<T, DP> S;
   typedef SeqCfg<T, DP> C;
-  int *tab = (int*)(smem_raw + S::RING), *flag = tab + SEQ_TAB, *red = flag + 4, *pre = flag + 16;  // pre[i]: steps of a head ahead of slot i
+  int *tab = (int*)(smem_raw + S::RING), *flag = tab + SEQ_TAB, *pre = flag + 16;  // pre[i]: parts of a head ahead of slot i
+  int* red = (int*)smem_raw;                                                       // sums of four waves, in the ring before it is used
   const SeqArgs& a = ra.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
-  // ---- steps of every slot
+  // ---- steps of every slot, PER of a thread
   for (int i = threadIdx.x; i <= a.n_seqs && i < SEQ_TAB; i += 256) tab[i] = a.offsets[i];
   __syncthreads();
   auto base_of = [&](int b) __attribute__((always_inline)) {
     const int o = b < SEQ_TAB ? tab[b] : a.offsets[b];
     return (int)((int64_t)(o < 0 ? 0 : (o > a.n_tokens ? a.n_tokens : o)) * a.group / S::BM) + b;
   };
-  const int per = (slots + 255) / 256, first = (int)threadIdx.x * per;
-  int mine = 0;
-  for (int i = first; i < first + per && i < slots; ++i) {
+  constexpr int PER = S::MOST / 256;
+  int steps[PER], all = 0, most = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * (int)threadIdx.x + j;
+    steps[j] = 0;
+    if (i >= slots) continue;
     int lo = 0, n = a.n_seqs;  // the last sequence whose base is at most i
     while (n > 1) {
       const int m = n / 2;
@@ -972,114 +1019,135 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
     }
     const SeqSpan sp = seq_span(a, lo);
     const int rows = sp.n * a.group, tiles = (rows + S::BM - 1) / S::BM, tile = tiles - 1 - (i - base_of(lo));
-    int steps = 0;
-    if (rows > 32 && tile >= 0 && tile < tiles) {
-      const int r1 = tile * S::BM + S::BM - 1 < rows ? tile * S::BM + S::BM - 1 : rows - 1;
-      const int p0 = sp.length - sp.n + tile * S::BM / a.group, p1 = sp.length - sp.n + r1 / a.group;
-      const int k0 = a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;
-      steps = (p1 + S::BN) / S::BN - k0 / S::BN;
-      if (p1 < 0 || steps < 1) steps = 1;  // no key at all: a step that writes the zeros
-    }
-    pre[i + 1] = mine += steps;
+    if (rows <= 32 || tile < 0 || tile >= tiles) continue;
+    const int r1 = tile * S::BM + S::BM - 1 < rows ? tile * S::BM + S::BM - 1 : rows - 1;
+    const int q0 = sp.length - sp.n + tile * S::BM / a.group, q1 = sp.length - sp.n + r1 / a.group;
+    const int k0 = a.window > 0 && q0 >= a.window ? q0 - a.window + 1 : 0;
+    steps[j] = (q1 + S::BN) / S::BN - k0 / S::BN;
+    if (q1 < 0 || steps[j] < 1) steps[j] = 1;  // no key at all: a step that writes the zeros
+    all += steps[j] < 1 << 20 ? steps[j] : 1 << 20;  // in 32 bits; a lower bound is all it is for
+    most = most > steps[j] ? most : steps[j];
   }
+  // a sum over the workgroup, the same in every lane
+  auto sum_of = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+    __syncthreads();
+    if (lane == 0) red[wave] = x;
+    __syncthreads();
+    return seq_same(red[0] + red[1] + red[2] + red[3]);
+  };
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_xor(most, d);
+    most = most > y ? most : y;
+  }
+  if (lane == 0) red[4 + wave] = most;
+  all = sum_of(all);
+  if (all == 0) return;
+  most = red[4] > red[5] ? red[4] : red[5];
+  most = most > red[6] ? most : red[6];
+  most = seq_same(most > red[7] ? most : red[7]);
+  // the least T: at least an even share, at most the longest tile, which makes a part of every tile
+  const int room = ra.shares / a.kv_heads;  // parts of a head
+  int lo = (all + room - 1) / room, hi = most;
+  lo = lo < S::LEAST ? S::LEAST : lo;
+  hi = hi > lo ? hi : lo;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) n += (steps[j] + mid - 1) / mid;
+    if (sum_of(n) <= room) hi = mid;
+    else lo = mid + 1;
+  }
+  int cut[PER], mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) mine += cut[j] = (steps[j] + lo - 1) / lo;
   int x = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
+  __syncthreads();
   if (lane == 63) red[wave] = x;
   __syncthreads();
   x -= mine;
   for (int w = 0; w < wave; ++w) x += red[w];
-  for (int i = first; i < first + per && i < slots; ++i) pre[i + 1] += x;
-  if (threadIdx.x == 0) pre[0] = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * (int)threadIdx.x + j;
+    if (i <= slots) pre[i] = x;
+    x += cut[j];
+  }
+  if (threadIdx.x == 255 && slots == S::MOST) pre[slots] = x;
   __syncthreads();
-  auto ahead = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(pre[i]); };
-  const int each = ahead(slots);
-  const int64_t total = (int64_t)each * a.kv_heads;
-  if (total == 0) return;
-  // ---- this workgroup's share: those of an XCD side by side, as their keys are
-  const int n_shares = seq_shares(total, ra.shares, S::LEAST), side = (n_shares + 7) / 8;
-  const int share = block % 8 * side + block / 8;
-  if (block / 8 >= side || share >= n_shares) return;
-  int64_t at = seq_share(total, n_shares, share);
-  const int64_t end = seq_share(total, n_shares, share + 1);
+  auto ahead = [&](int i) __attribute__((always_inline)) { return seq_same(pre[i]); };
+  const int each = ahead(slots), parts_all = each * a.kv_heads;
+  // ---- this workgroup's part: those of an XCD side by side, as their keys are
+  const int side = (parts_all + 7) / 8, part = block % 8 * side + block / 8;
+  if (block / 8 >= side || part >= parts_all) return;
+  const int head = part / each, r = part - head * each;
   int slot = 0;
-  {  // the slot of the first step
-    const int r = (int)(at % each);
-    int n = slots;
-    while (n > 1) {
-      const int m = n / 2;
-      if (ahead(slot + m) <= r) {
-        slot += m;
-        n -= m;
-      } else {
-        n = m;
-      }
+  for (int n = slots; n > 1;) {
+    const int m = n / 2;
+    if (ahead(slot + m) <= r) {
+      slot += m;
+      n -= m;
+    } else {
+      n = m;
     }
   }
-  int head = (int)(at / each);
-  while (at < end) {
-    while (ahead(slot + 1) == ahead(slot) || (int64_t)head * each + ahead(slot + 1) <= at)
-      if (++slot == slots) {
-        slot = 0;
-        ++head;
-      }
-    const int64_t s0 = (int64_t)head * each + ahead(slot);
-    const int steps = ahead(slot + 1) - ahead(slot), ta = (int)(at - s0), tb = steps - ta < end - at ? steps : ta + (int)(end - at);
-    at += tb - ta;
-    SeqTile s;
-    (void)seq_tile<S::BM, S::BN, true>(a, slot, head, s, wave, lane);
-    if (threadIdx.x == 0) flag[1] = s.x.bad;
-    SeqState<T, DP> st;
-    st.load_q(a.q + (s.sp.first + s.token) * a.q_token + s.h * a.q_head, lane >> 5, a.kchunks);
-    st.clear();
-    const int t1 = s.t_lo + tb < s.t_hi ? s.t_lo + tb : s.t_hi;
-    seq_tile_run<T, DP, true>(a, s, st, s.t_lo + ta, t1, lds0, tab, flag + 1, wave, lane);
+  const int parts = ahead(slot + 1) - ahead(slot), p = r - ahead(slot);
+  SeqTile s;
+  if (!seq_tile<S::BM, S::BN, true>(a, slot, head, s, wave, lane)) return;  // offsets that do not ascend: none of the tile's parts runs
+  if (threadIdx.x == 0) flag[1] = s.x.bad;
+  SeqState<T, DP> st;
+  st.load_q(a.q + (s.sp.first + s.token) * a.q_token + s.h * a.q_head, lane >> 5, a.kchunks);
+  st.clear();
+  const int n = s.t_hi > s.t_lo ? s.t_hi - s.t_lo : 0;
+  __syncthreads();  // the sums in the ring are read
+  auto border = [&](int i) __attribute__((always_inline)) { return s.t_lo + (int)((int64_t)n * i / parts); };
+  seq_tile_run<T, DP, true>(a, s, st, border(p), border(p + 1), lds0, tab, flag + 1, wave, lane);
+  __syncthreads();
+  float l = flag[1] ? NAN : xor32_sum(st.l);
+  if (parts > 1) {
+    const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64, first = part - p;  // pitch of a wave
+    auto at = [&](int i) __attribute__((always_inline)) { return ra.ws_tiles + (size_t)(first + i) * 4 * pitch + wave * pitch + lane; };
+    float* to = at(p);
+#pragma unroll
+    for (int n = 0; n < C::NMB; ++n)
+      if (n < blocks)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) seq_give(to + (16 * n + i) * 64, st.o[n][i]);
+    seq_give(to + (16 * blocks) * 64, st.m);
+    seq_give(to + (16 * blocks + 1) * 64, l);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
     __syncthreads();
-    float l = flag[1] ? NAN : xor32_sum(st.l);
-    if (ta != 0 || tb != steps) {
-      const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64;  // of a wave
-      const int i0 = seq_owner(total, n_shares, s0), parts = seq_owner(total, n_shares, s0 + steps - 1) - i0 + 1;
-      float* to = ra.ws_tiles + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
+    if (threadIdx.x == 0) {
+      flag[0] = __hip_atomic_fetch_add(&ra.brought_tiles[first], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+      if (flag[0]) __hip_atomic_store(&ra.brought_tiles[first], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!seq_same(flag[0])) return;
+    float m = -INFINITY;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, seq_take(at(i) + (16 * blocks) * 64));
+    st.clear();
+    l = 0.f;
+    for (int i = 0; i < parts; ++i) {
+      const float* from = at(i);
+      const float mp = seq_take(from + (16 * blocks) * 64), lp = seq_take(from + (16 * blocks + 1) * 64);
+      const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
+      l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
 #pragma unroll
       for (int n = 0; n < C::NMB; ++n)
         if (n < blocks)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) seq_give(to + (16 * n + i) * 64, st.o[n][i]);
-      seq_give(to + (16 * blocks) * 64, st.m);
-      seq_give(to + (16 * blocks + 1) * 64, l);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        flag[0] = __hip_atomic_fetch_add(&ra.brought_tiles[i0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
-        if (flag[0]) __hip_atomic_store(&ra.brought_tiles[i0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (!__builtin_amdgcn_readfirstlane(flag[0])) continue;
-      // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
-      auto part = [&](int p) __attribute__((always_inline)) {
-        return ra.ws_tiles + (size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 4 * pitch + wave * pitch + lane;
-      };
-      float m = -INFINITY;
-      for (int p = 0; p < parts; ++p) m = fmaxf(m, seq_take(part(p) + (16 * blocks) * 64));
-      st.clear();
-      l = 0.f;
-      for (int p = 0; p < parts; ++p) {
-        const float* from = part(p);
-        const float mp = seq_take(from + (16 * blocks) * 64), lp = seq_take(from + (16 * blocks + 1) * 64);
-        const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
-        l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
-#pragma unroll
-        for (int n = 0; n < C::NMB; ++n)
-          if (n < blocks)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[n][i] = __builtin_fmaf(seq_take(from + (16 * n + i) * 64), f, st.o[n][i]);
-      }
+          for (int j = 0; j < 16; ++j) st.o[n][j] = __builtin_fmaf(seq_take(from + (16 * n + j) * 64), f, st.o[n][j]);
     }
-    seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
   }
+  seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
 }
 
 // Sequences of many rows and of few at once: workgroups for the tiles of the one, behind them those for the keys of the other.  At heads

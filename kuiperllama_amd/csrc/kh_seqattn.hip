@@ -17,8 +17,9 @@ int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
     return KH_ERR_INVALID_ARG;
   const int e = *esize = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
   if (!whole(r->head_size, e) || !whole(r->value_size, e) || r->head_size > 256 || r->value_size > 256) return KH_ERR_UNSUPPORTED;
-  // rows of a sequence are counted in 32 bits, and so are the workgroups
-  if ((int64_t)r->n_tokens * r->head_num > INT_MAX / 2 || r->n_seqs > INT_MAX / 2 / r->kv_head_num) return KH_ERR_UNSUPPORTED;
+  // rows of a sequence are counted in 32 bits, and a grid has 2^32 threads
+  if ((int64_t)r->n_tokens * r->head_num > INT_MAX / 2 || (int64_t)r->n_tokens * r->head_num / 128 + (int64_t)r->n_seqs * r->kv_head_num >= 1 << 24)
+    return KH_ERR_UNSUPPORTED;
   if (r->n_tokens == 0 || r->n_seqs == 0) return KH_OK;
   if (!r->offsets || !r->q || !r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !whole(r->q_token, e) || !whole(r->q_head, e) ||
       !whole(r->o_token, e) || !whole(r->o_head, e))
@@ -63,13 +64,20 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   typedef SeqTiles<T, DP> S;
   typedef SeqRows<T, DP> R;
   typedef SeqMixed<T, DP> M;
+  constexpr int CB = SeqCfg<T, DP>::CB;
+  const SeqKv& kv = a.s.kv;
+  auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 24; };  // 64 rows apart in 32 bits
+  a.s.kv.plain = a.s.kchunks == CB && a.s.vchunks == CB && near(kv.k_slot) && near(kv.v_slot) && (!kv.pages || kv.page_size % (64 / CB) == 0);
   a.shares = R::SHARES;
   a.all = how == FEW;
   if (how == FEW) return launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
   const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
   const dim3 grid((unsigned)(slots * a.s.kv_heads));
   if (how == PACKED) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
-  if (slots <= S::MOST && slots * a.s.kv_heads <= 4 * M::SHARES) {
+  // Tiles that are fewer than the workgroups the chip holds are cut along their keys (136 tiles of 512 tokens behind 16384 keys: 345 us,
+  // 1214 whole; 16 of 64 behind 4096: 33, 81); as many or more are left whole (520 of 2048 tokens behind 8192: 290 us, 333 with
+  // cuts).
+  if (slots <= S::MOST && slots * a.s.kv_heads <= M::SHARES) {
     a.shares = M::SHARES;
     a.brought_tiles = a.brought + SEQ_SHARES;
     a.ws_tiles = a.ws + (size_t)2 * SEQ_SHARES * 32 * (a.s.vchunks * (16 / (int)sizeof(T)) + 4);
@@ -111,9 +119,10 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
 
 extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens) {
   if (head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || value_size <= 0 || n_tokens < 0) return KH_ERR_INVALID_ARG;
-  // counters, and two parts of a share: 32 rows, and 128 as four waves hold them where a call can have as many
+  // counters, two parts of 32 rows a share, and one of 128 rows as four waves hold them where a call can have as many
   const bool tiles = (int64_t)n_tokens * (head_num / kv_head_num) > 32;
-  return 4 * (2 * khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * (32 * ((int64_t)value_size + 4) + (tiles ? (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0)));
+  return 4 * (2 * khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * 32 * ((int64_t)value_size + 4) +
+              (tiles ? khm::SEQ_SHARES * (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0));
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
