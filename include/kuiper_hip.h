@@ -163,7 +163,8 @@ int kh_scale_sum_f32(const float* value, const float* scale, float* out, int32_t
  * head h goes with key head h / (head_num / kv_head_num).
  *
  * Types: KH_DTYPE_BF16, KH_DTYPE_F32 (sums, softmax and angles in fp32 or more either way).  Pointers are aligned to 16
- * bytes; head sizes and strides are multiples of 16 bytes; head_size and value_size are at most 256.  Anything else is refused:
+ * bytes; head sizes and strides are multiples of 16 bytes; head_size and value_size are at most 256, a rotation has
+ * fewer than 2^24 tokens, attention fewer than 2^30 query rows (tokens times heads).  Anything else is refused:
  * KH_ERR_INVALID_ARG, KH_ERR_UNSUPPORTED for the sizes.  No tokens or no sequences: nothing is done.
  *
  * A cache of pages: token j of a sequence lies in slot j % page_size of page pages[seq][j / page_size].  Pages may lie in
@@ -179,7 +180,7 @@ typedef struct kh_page_cache {
  *   BANDS   pairs of more than `high` turns within `original` positions stay, those of fewer than `low` are divided by
  *           factor, in between the two are mixed linearly in the number of turns
  *   RAMP    the same idea over the pair's number: from floor(pair of `fast` turns) to ceil(pair of `slow` turns); rotated pairs
- *           are multiplied by `magnitude` (0: 0.1 ln factor + 1)
+ *           are multiplied by `magnitude` (0: 0.1 ln factor + 1, or 1 for factors below 1)
  * turns[i] = freq_i / 2 pi as a 64-bit fraction of a turn: position * turns modulo 2^64 is the angle modulo a turn, off by at
  * most |position| 2^-54 turns (host-only; the caller copies the table to the device). */
 enum { KH_ROPE_SCALE_NONE = 0, KH_ROPE_SCALE_LINEAR = 1, KH_ROPE_SCALE_BANDS = 2, KH_ROPE_SCALE_RAMP = 3 };
@@ -191,7 +192,7 @@ int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scaling* scaling 
                   float* h_magnitude);
 
 /* The first rot_dim elements of every head are rotated by their token's position (any int32), the others pass; mode as in
- * kh_rope_f32.  q_out / k_out may be q / k (with the same strides); they may not overlap them otherwise. */
+ * kh_rope_f32.  q_out / k_out may be q / k, with the same strides (refused with others); they may not overlap them otherwise. */
 typedef struct kh_rope_rows {
   int32_t dtype, mode, n_tokens, head_num, kv_head_num, head_size, rot_dim;
   float magnitude;
@@ -219,7 +220,7 @@ typedef struct kh_attn_rows {
   const int32_t* offsets;     /* [n_seqs + 1], ascending, at most n_tokens */
   const void* q;              /* [n_tokens][head_num][head_size] */
   int64_t q_token, q_head;
-  void* out;                  /* [n_tokens][head_num][value_size]; may not overlap q */
+  void* out;                  /* [n_tokens][head_num][value_size]; may not overlap q (refused where it is q) */
   int64_t o_token, o_head;
 } kh_attn_rows;
 /* Whole prompts: the keys and values of a sequence are the rows of its own tokens. */

@@ -220,9 +220,17 @@ int check_rows(const kh_rope_rows* r, bool store) {
     return KH_ERR_INVALID_ARG;
   const int e = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
   if (!whole(r->head_size, e) || r->head_size > 256 || r->n_tokens >= 1 << 24) return KH_ERR_UNSUPPORTED;  // a grid has 2^32 threads
+  if (r->n_tokens == 0) return KH_OK;
   if ((r->rot_dim && !r->turns) || !r->positions || !r->q || !r->k || !r->q_out || (!store && !r->k_out) || !kh_aligned16(r->q) || !kh_aligned16(r->k) ||
       !kh_aligned16(r->q_out) || (!store && !kh_aligned16(r->k_out)) || !whole(r->q_token, e) || !whole(r->q_head, e) || !whole(r->k_token, e) ||
       !whole(r->k_head, e) || !whole(r->qo_token, e) || !whole(r->qo_head, e) || (!store && (!whole(r->ko_token, e) || !whole(r->ko_head, e))))
+    return KH_ERR_INVALID_ARG;
+  // in place: a row is written where it was read
+  auto moved = [&](int64_t token, int64_t head, int64_t o_token, int64_t o_head, int heads) {
+    return (token != o_token && r->n_tokens > 1) || (head != o_head && heads > 1);
+  };
+  if ((r->q == r->q_out && moved(r->q_token, r->q_head, r->qo_token, r->qo_head, r->head_num)) ||
+      (!store && r->k == r->k_out && moved(r->k_token, r->k_head, r->ko_token, r->ko_head, r->kv_head_num)))
     return KH_ERR_INVALID_ARG;
   return KH_OK;
 }
@@ -295,7 +303,7 @@ extern "C" int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scalin
     hi = ceil(pair(c->slow));
     lo = lo > 0 ? lo : 0;
     hi = hi < rot_dim - 1 ? hi : rot_dim - 1;
-    *h_magnitude = (float)(c->magnitude > 0 ? c->magnitude : 0.1 * log(c->factor) + 1.0);
+    *h_magnitude = (float)(c->magnitude > 0 ? c->magnitude : (c->factor > 1 ? 0.1 * log(c->factor) + 1.0 : 1.0));
   }
   for (int i = 0; i < rot_dim / 2; ++i) {
     double f = pow(theta, -2.0 * i / rot_dim);
@@ -332,11 +340,11 @@ extern "C" int kh_rope_store(const kh_rope_rows* r, const void* v, int64_t v_tok
   const int e = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
   if (value_size <= 0) return KH_ERR_INVALID_ARG;
   if (!khm::whole(value_size, e) || value_size > 256) return KH_ERR_UNSUPPORTED;
+  if (r->n_tokens == 0) return KH_OK;
   if (!v || !c || !slots || !c->k || !c->v || c->n_pages <= 0 || c->page_size <= 0 || !kh_aligned16(v) || !kh_aligned16(c->k) ||
       !kh_aligned16(c->v) || !khm::whole(v_token, e) || !khm::whole(v_head, e) || !khm::whole(c->k_page, e) || !khm::whole(c->k_slot, e) ||
       !khm::whole(c->k_head, e) || !khm::whole(c->v_page, e) || !khm::whole(c->v_slot, e) || !khm::whole(c->v_head, e))
     return KH_ERR_INVALID_ARG;
-  if (r->n_tokens == 0) return KH_OK;
   return r->dtype == KH_DTYPE_BF16 ? khm::store<khm::bf16>(r, v, v_token, v_head, value_size, c, slots, (hipStream_t)stream)
                                    : khm::store<float>(r, v, v_token, v_head, value_size, c, slots, (hipStream_t)stream);
 }

@@ -21,7 +21,7 @@ int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
   if ((int64_t)r->n_tokens * r->head_num > INT_MAX / 2 || (int64_t)r->n_tokens * r->head_num / 128 + (int64_t)r->n_seqs * r->kv_head_num >= 1 << 24)
     return KH_ERR_UNSUPPORTED;
   if (r->n_tokens == 0 || r->n_seqs == 0) return KH_OK;
-  if (!r->offsets || !r->q || !r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !whole(r->q_token, e) || !whole(r->q_head, e) ||
+  if (!r->offsets || !r->q || !r->out || r->q == r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !whole(r->q_token, e) || !whole(r->q_head, e) ||
       !whole(r->o_token, e) || !whole(r->o_head, e))
     return KH_ERR_INVALID_ARG;
   *todo = 1;

@@ -7,6 +7,7 @@ torch's current stream.  There is no eager/CPU fallback: a CPU tensor is an erro
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import NamedTuple, Optional
 
@@ -204,18 +205,27 @@ def rope_turns(rot_dim: int, theta: float, scaling: Optional[dict] = None):
     """(fractions of a turn a position, of 2**64, for each of rot_dim / 2 pairs; factor of rotated pairs).  scaling: as rope_scaling in
     a model's config.json, rope_type "default", "linear", "llama3" or "yarn"."""
     import ctypes as C
-    c, kind = None, (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
-    if kind == "linear":
-        c = _ffi.RopeScaling(kind=1, factor=scaling["factor"])
-    elif kind == "llama3":
-        c = _ffi.RopeScaling(kind=2, factor=scaling["factor"], original=scaling["original_max_position_embeddings"],
-                             low=scaling["low_freq_factor"], high=scaling["high_freq_factor"])
-    elif kind == "yarn":
-        c = _ffi.RopeScaling(kind=3, factor=scaling["factor"], original=scaling["original_max_position_embeddings"],
-                             fast=scaling.get("beta_fast", 32.0), slow=scaling.get("beta_slow", 1.0),
-                             magnitude=scaling.get("attention_factor") or 0.0)
-    elif kind != "default":
-        raise ValueError(f"rope_type {kind!r}: default, linear, llama3 or yarn expected")
+    given, c = scaling or {}, None
+    kind = given.get("rope_type", given.get("type", "default"))
+    try:
+        if kind == "linear":
+            c = _ffi.RopeScaling(kind=1, factor=given["factor"])
+        elif kind == "llama3":
+            c = _ffi.RopeScaling(kind=2, factor=given["factor"], original=given["original_max_position_embeddings"],
+                                 low=given["low_freq_factor"], high=given["high_freq_factor"])
+        elif kind == "yarn":
+            if given.get("truncate") is False:
+                raise ValueError("yarn with borders between pairs (truncate: false) is not supported")
+            factor, magnitude = given["factor"], given.get("attention_factor")
+            if not magnitude and given.get("mscale") and given.get("mscale_all_dim"):
+                one, all_dims = (0.1 * given[n] * math.log(max(factor, 1.0)) + 1.0 for n in ("mscale", "mscale_all_dim"))
+                magnitude = one / all_dims
+            c = _ffi.RopeScaling(kind=3, factor=factor, original=given["original_max_position_embeddings"],
+                                 fast=given.get("beta_fast") or 32.0, slow=given.get("beta_slow") or 1.0, magnitude=magnitude or 0.0)
+        elif kind != "default":
+            raise ValueError(f"rope_type {kind!r}: default, linear, llama3 or yarn expected")
+    except KeyError as e:
+        raise KeyError(f"rope_type {kind!r} needs {e}") from None
     turns, magnitude = (C.c_uint64 * max(1, rot_dim // 2))(), C.c_float()
     _ffi.check(_ffi.lib().kh_rope_turns(rot_dim, theta, C.byref(c) if c is not None else None, turns, C.byref(magnitude)), "kh_rope_turns")
     return list(turns)[:rot_dim // 2], magnitude.value

@@ -32,7 +32,7 @@ def cache(**kw):
 
 def attn_rows(**kw):
     r = dict(dtype=1, n_tokens=4, n_seqs=2, head_num=4, kv_head_num=2, head_size=64, value_size=64, window=0, scale=0.125, offsets=P, q=P,
-             q_token=256, q_head=64, out=P, o_token=256, o_head=64)
+             q_token=256, q_head=64, out=2 * P, o_token=256, o_head=64)
     r.update(kw)
     return _ffi.AttnRows(**r)
 
@@ -107,6 +107,36 @@ def test_nothing_to_do_is_no_error(lib):
         assert lib.kh_attn_paged(C.byref(attn_rows(**kw)), C.byref(cache()), P, 4, 4, P, 0, P, 1 << 40, None) == 0
 
 
+def test_nothing_to_do_needs_no_addresses(lib):
+    """An empty tensor has none."""
+    none = dict(turns=None, positions=None, q=None, k=None, q_out=None)
+    assert lib.kh_rope_tokens(C.byref(rope_rows(n_tokens=0, k_out=None, **none)), None) == 0
+    assert lib.kh_rope_store(C.byref(rope_rows(n_tokens=0, **none)), None, 128, 64, 64, C.byref(cache()), None, None) == 0
+    r = C.byref(attn_rows(n_tokens=0, q=None, out=None, offsets=None))
+    assert lib.kh_attn_packed(r, None, 128, 64, None, 128, 64, None) == 0
+    assert lib.kh_attn_paged(r, C.byref(cache()), None, 4, 4, None, 0, None, 0, None) == 0
+
+
+def test_places_that_overlap_are_refused(lib):
+    """Results where rows are still to be read: in place with other strides, an output that is the queries."""
+    other = P + 4096
+    for at, to in (("q_token", "qo_token"), ("q_head", "qo_head"), ("k_token", "ko_token"), ("k_head", "ko_head")):
+        r = rope_rows(**{to: 8 * getattr(rope_rows(), at)})
+        assert lib.kh_rope_tokens(C.byref(r), None) == -1, at
+        if at[0] == "q":
+            assert lib.kh_rope_store(C.byref(r), P, 128, 64, 64, C.byref(cache()), P, None) == -1, at
+    r = C.byref(attn_rows(out=P))  # q too
+    assert lib.kh_attn_packed(r, other, 128, 64, other, 128, 64, None) == -1
+    assert lib.kh_attn_paged(r, C.byref(cache()), P, 4, 4, P, 0, P, 1 << 40, None) == -1
+
+
+def test_launches_that_no_grid_holds(lib):
+    assert lib.kh_rope_tokens(C.byref(rope_rows(n_tokens=1 << 24)), None) == _ffi.KH_ERR_UNSUPPORTED
+    assert lib.kh_rope_store(C.byref(rope_rows(n_tokens=1 << 24)), P, 128, 64, 64, C.byref(cache()), P, None) == _ffi.KH_ERR_UNSUPPORTED
+    for kw in (dict(n_seqs=1 << 23), dict(n_tokens=1 << 28)):
+        assert lib.kh_attn_packed(C.byref(attn_rows(**kw)), P, 128, 64, P, 128, 64, None) == _ffi.KH_ERR_UNSUPPORTED, kw
+
+
 def test_workspace_sizes(lib):
     for bad in ((0, 1, 64, 1), (4, 3, 64, 1), (4, 2, 0, 1), (4, 2, 64, -1)):
         assert lib.kh_attn_paged_workspace_bytes(*bad) == -1, bad
@@ -167,6 +197,21 @@ def test_turns(rot, theta, scaling):
     for t, f in zip(turns, want):
         # a few roundings of 64 bits each side: pow, products, the quotient by 2 pi
         assert abs(t / 2 ** 64 - f / (2 * math.pi) % 1.0) <= 16 * 2 ** -53 * f / (2 * math.pi) + 2 ** -64
+
+
+def test_yarn_s_factor():
+    """Of the two factors of a model with latent keys; 1 where nothing is stretched; refused where the borders are no pairs."""
+    yarn = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+    factor = lambda **kw: ops.rope_turns(64, 1e4, {**yarn, **kw})[1]  # noqa: E731
+    assert factor(mscale=0.707, mscale_all_dim=1.0) == pytest.approx((0.0707 * math.log(40) + 1) / (0.1 * math.log(40) + 1), rel=2 ** -23)
+    assert factor(mscale=1.0, mscale_all_dim=1.0) == 1.0
+    assert factor(mscale=0.707) == factor(attention_factor=None) == pytest.approx(0.1 * math.log(40) + 1, rel=2 ** -23)
+    assert factor(mscale=0.5, mscale_all_dim=1.0, attention_factor=1.5) == 1.5
+    assert factor(factor=0.5) == 1.0
+    with pytest.raises(ValueError, match="truncate"):
+        factor(truncate=False)
+    with pytest.raises(KeyError, match="original_max_position_embeddings"):
+        ops.rope_turns(64, 1e4, {"rope_type": "yarn", "factor": 40.0})
 
 
 def test_turns_refuse(lib):

@@ -422,6 +422,146 @@ def test_a_layer_s_attention_in_portions(gpu, dtype):
         done = [n + 1 for n in done]
 
 
+# ---- units and tiles that are cut: long keys, few sequences ------------------------------------------------------------------
+CUT = [  # heads, kv_heads, key size, value size, new tokens, lengths, page: single tokens dealt by steps of keys, portions cut into parts
+    (8, 1, 64, 64, [1], [20000], 16), (4, 1, 128, 128, [2, 1], [9000, 5], 16), (2, 1, 256, 256, [1], [3000], 32), (4, 2, 48, 80, [1, 3], [2500, 1], 8),
+    (8, 1, 64, 64, [200], [6000], 3), (4, 2, 128, 128, [300, 1], [4000, 2000], 16), (4, 1, 256, 256, [60, 40, 1], [1500, 2100, 700], 32),
+    (8, 2, 128, 96, [257], [1700], 24)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", CUT, ids=lambda c: str(c)[:60])
+def test_cut_keys(gpu, dtype, case):
+    """Against the formula; a page that is none in one of the parts; values that are no numbers in keys that some rows do not see."""
+    from kuiperllama_amd import ops
+    H, KH, D, DV, new, lens, page = case
+    gen = generator(sum(lens) + D)
+    kc, vc, table, ks, vs = paged(gen, dtype, KH, D, DV, lens, page)
+    T = sum(new)
+    q = rnd(gen, dtype, T, H, D, scale=1.5)
+    lengths, off = torch.tensor(lens, dtype=torch.int32, device=gpu), offsets_of(new, gpu)
+    ws = ops.attn_paged_workspace(H, KH, DV, T, gpu)
+
+    def run(pages):
+        out = torch.full((T, H, DV), 9.0, dtype=dtype, device=gpu)
+        return ops.attn_paged(q, kc, vc, pages, lengths, off, out, ws)
+
+    good = run(table)
+    check_paged(q, good, lens, new, ks, vs, 0)
+    assert torch.equal(run(table), good)
+    for at in (1, lens[0] // page // 2):  # of the first sequence
+        broken = table.clone()
+        broken[0, at] = -5
+        out = run(broken)
+        assert torch.isnan(out[:new[0]]).all() and torch.equal(out[new[0]:], good[new[0]:])
+    assert torch.equal(run(table), good)
+    # the last token of the first sequence, and one in the middle of its new ones, hold what is no number
+    n, length = new[0], lens[0]
+    spoilt = torch.zeros(T, H, DV, dtype=torch.bool, device=gpu)
+    for place, value in ((length - 1, math.nan), (length - 1 - n // 2, -math.inf)):
+        pg = int(table[0, place // page])
+        vc[pg, place % page, 0, ::3] = value
+        spoilt[max(0, place - (length - n)):n, :H // KH, ::3] = True
+    out = run(table)
+    assert not torch.isfinite(out[spoilt]).any()
+    want, bound = attended(q[:n], ks[0], vs[0], 0, D ** -0.5)
+    close(out[:n][~spoilt[:n]], want[~spoilt[:n]], bound[~spoilt[:n]], "beside what is no number")
+    assert torch.equal(out[n:], good[n:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 1], [70, 1, 40]], ids=str)
+def test_one_cache_tensor_and_a_window(gpu, dtype, new):
+    """Keys and values side by side in one tensor, queries a slice of wider rows, every length of the last page."""
+    from kuiperllama_amd import ops
+    gen = generator(31 + sum(new))
+    H, KH, D, page, window = 6, 2, 64, 16, 50
+    T = sum(new)
+    for extra in range(0, page, 5):
+        lens = [300 + extra, max(new[1], 33) + extra, 41 + extra]
+        kc, vc, table, ks, vs = paged(gen, dtype, KH, D, D, lens, page)
+        both = torch.stack([kc, vc], 2)  # [pages, page, 2, kv_heads, size]
+        rows = rnd(gen, dtype, T, 2, H, D)
+        out = torch.full((T, 2, H, D), 9.0, dtype=dtype, device=gpu)
+        ops.attn_paged(rows[:, 1], both[:, :, 0], both[:, :, 1], table, torch.tensor(lens, dtype=torch.int32, device=gpu), offsets_of(new, gpu), out[:, 0],
+                       ops.attn_paged_workspace(H, KH, D, T, gpu), window=window)
+        check_paged(rows[:, 1], out[:, 0], lens, new, ks, vs, window, f"extra {extra}")
+        assert (out[:, 1] == 9.0).all()
+
+
+def test_keys_that_heads_share_by_a_stride_of_zero(gpu):
+    from kuiperllama_amd import ops
+    gen = generator(6)
+    q, k, v = rnd(gen, BF16, 90, 4, 64), rnd(gen, BF16, 90, 1, 64), rnd(gen, BF16, 90, 1, 64)
+    a, b = (ops.attn_packed(q, x, y, offsets_of([70, 20], gpu), torch.empty_like(q)) for x, y in ((k, v), (k.expand(-1, 4, -1), v.expand(-1, 4, -1))))
+    close(a[:70], *attended(q[:70], k[:70], v[:70], 0, 0.125))
+    close(b[:70], *attended(q[:70], k[:70], v[:70], 0, 0.125))
+    close(b[70:], *attended(q[70:], k[70:], v[70:], 0, 0.125))
+
+
+def test_no_tokens(gpu):
+    from kuiperllama_amd import ops
+    f = lambda *s: torch.zeros(*s, dtype=BF16, device=gpu)  # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=gpu)  # noqa: E731
+    table = ops.rope_table(64, 1e4, gpu)
+    ops.rope_tokens(f(0, 4, 64), f(0, 2, 64), i(0), table, 1)
+    ops.rope_store(f(0, 4, 64), f(0, 2, 64), f(0, 2, 64), i(0), table, 1, f(3, 16, 2, 64), f(3, 16, 2, 64), i(0))
+    ops.attn_packed(f(0, 4, 64), f(0, 2, 64), f(0, 2, 64), i(1), f(0, 4, 64))
+    ws = ops.attn_paged_workspace(4, 2, 64, 0, gpu)
+    ops.attn_paged(f(0, 4, 64), f(3, 16, 2, 64), f(3, 16, 2, 64), i(2, 3), i(2), i(3), f(0, 4, 64), ws)
+    out = f(5, 4, 64) + 9  # a padded batch of no sequence
+    ops.attn_packed(f(5, 4, 64), f(5, 2, 64), f(5, 2, 64), i(1), out)
+    ops.attn_paged(f(5, 4, 64), f(3, 16, 2, 64), f(3, 16, 2, 64), i(0, 3), i(0), i(1), out, ops.attn_paged_workspace(4, 2, 64, 5, gpu))
+    assert (out == 9).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_one_workspace_for_calls_of_any_shape(gpu, dtype):
+    """Two captured graphs and eager calls of other shapes, one after the other, over one workspace; lengths move between replays."""
+    from kuiperllama_amd import ops
+    gen = generator(55)
+    KH, D, page = 2, 64, 16
+    lens = [[2000, 5, 900], [1500, 2500]]
+    news = [[1, 1, 1], [90, 40]]
+    caches = [paged(gen, dtype, KH, D, D, n, page) for n in lens]
+    qs = [rnd(gen, dtype, sum(n), 8, D) for n in news]
+    ws = ops.attn_paged_workspace(8, KH, D, 130, gpu)
+    lengths = [torch.tensor(n, dtype=torch.int32, device=gpu) for n in lens]
+    offs = [offsets_of(n, gpu) for n in news]
+    outs = [torch.zeros_like(q) for q in qs]
+
+    def call(i, out):
+        kc, vc, table = caches[i][:3]
+        ops.attn_paged(qs[i], kc, vc, table, lengths[i], offs[i], out, ws, max_new=max(news[i]))
+
+    for i in range(2):
+        call(i, outs[i])
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i, outs[i])
+        graphs.append(g)
+    for turn in range(6):
+        now = [[n - 13 * turn if n > 100 else n for n in x] for x in lens]
+        for i in range(2):
+            lengths[i].copy_(torch.tensor(now[i], dtype=torch.int32))
+            outs[i].fill_(math.nan)
+        order = (0, 1) if turn % 2 else (1, 0)
+        for i in order:
+            graphs[i].replay()
+        eager = [torch.zeros_like(o) for o in outs]
+        for i in order:
+            call(i, eager[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], eager[i]), turn
+            ks, vs = ([x[:n] for x, n in zip(t, now[i])] for t in caches[i][3:])
+            check_paged(qs[i], outs[i], now[i], news[i], ks, vs, 0, f"turn {turn}")
+    assert not ws[:4096].any()  # the counters, as the next call needs them
+
+
 def test_another_stream_and_the_same_answer_twice(gpu):
     from kuiperllama_amd import ops
     gen = generator(12)
