@@ -377,7 +377,7 @@ struct SeqTiles {
   static constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   static constexpr int TB = BN * SeqCfg<T, DP>::RB;  // bytes of a tile of keys
   static constexpr int RING = 4 * TB;                // two tiles of keys and values each
-  static constexpr int MOST = 512;                   // slots that are looked at to be cut
+  static constexpr int MOST = 1024;                  // slots that are looked at to be cut
   static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
   static constexpr int LEAST = 512 / BN;             // steps of a part
 };
@@ -572,7 +572,7 @@ struct SeqRowsArgs {
   // [N] parts brought of the unit that begins in workgroup i's share and ends behind it, 0 between launches
   int* brought;
   float* ws;        // [2 N][32][value size + 4], o, m, l: of the unit that began before workgroup i's share, of the one that ends behind it
-  int shares, all;  // N; all: sequences of more than 32 rows too, 32 at a time
+  int all;          // sequences of more than 32 rows too, 32 at a time
   // the same for tiles of many rows
   int* brought_tiles;
   float* ws_tiles;
@@ -756,9 +756,9 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
   return odd;
 }
 
-// Workgroup `share` of k_seq_rows
+// Workgroup `share` of `shares`
 template <class T, int DP>
-__device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char* smem_raw) {
+__device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int share, char* smem_raw) {
   typedef SeqRows<T, DP> S;
   typedef SeqCfg<T, DP> C;
   int* tab = (int*)(smem_raw + S::RING);
@@ -771,7 +771,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
   const unsigned ring = lds0 + (unsigned)(wave * S::NB * S::TB);
   // ---- this workgroup's share
   const SeqScan sc = seq_scan(ra, red);
-  const int n_shares = seq_shares(sc.total, ra.shares);
+  const int n_shares = seq_shares(sc.total, shares);
   if (share >= n_shares) return;
   int64_t at = seq_share(sc.total, n_shares, share);
   const int64_t end = seq_share(sc.total, n_shares, share + 1);
@@ -975,17 +975,17 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int share, char*
 template <class T, int DP>
 __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  seq_rows<T, DP>(a, blockIdx.x, smem_raw);
+  seq_rows<T, DP>(a, SeqRows<T, DP>::SHARES, blockIdx.x, smem_raw);
 }
 
 // ---- many rows, few tiles ----------------------------------------------------------------------------------------------------------
 // Tiles of 128 rows over long keys that are too few for the chip - a portion of a prompt behind a long context - are cut along their
 // keys: every tile into as many equal parts of at most T steps as it takes, with the least T whose parts are no more than the workgroups
-// that fit on the chip at once.  (Dealt like the units above, at borders wherever they fall, a workgroup has two parts to hand over and
+// that fit on the chip at once; whole, where there are more tiles than those.  (Dealt like the units above, at borders wherever they fall, a workgroup has two parts to hand over and
 // not one: 64 KB each, 8 x 256 tokens behind 1792 keys 138 us, 91 where no tile is cut.)  A part lies in the workspace as it lay in the
 // registers ([wave][o ..., m, l][lane]), so that the workgroup that adds the parts, the last one to bring one, reads it lane by lane.
 template <class T, int DP>
-__device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots, int block, char* smem_raw) {
+__device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots, int shares, int block, char* smem_raw) {
   typedef SeqTiles<T, DP> S;
   typedef SeqCfg<T, DP> C;
   int *tab = (int*)(smem_raw + S::RING), *flag = tab + SEQ_TAB, *pre = flag + 16;  // pre[i]: parts of a head ahead of slot i
@@ -993,7 +993,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   const SeqArgs& a = ra.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
-  // ---- steps of every slot, PER of a thread
+  // ---- steps of every slot, slot i a thread's of number i mod 256
   for (int i = threadIdx.x; i <= a.n_seqs && i < SEQ_TAB; i += 256) tab[i] = a.offsets[i];
   __syncthreads();
   auto base_of = [&](int b) __attribute__((always_inline)) {
@@ -1004,7 +1004,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   int steps[PER], all = 0, most = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const int i = PER * (int)threadIdx.x + j;
+    const int i = 256 * j + (int)threadIdx.x;
     steps[j] = 0;
     if (i >= slots) continue;
     int lo = 0, n = a.n_seqs;  // the last sequence whose base is at most i
@@ -1049,7 +1049,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   most = most > red[6] ? most : red[6];
   most = seq_same(most > red[7] ? most : red[7]);
   // the least T: at least an even share, at most the longest tile, which makes a part of every tile
-  const int room = ra.shares / a.kv_heads;  // parts of a head
+  const int room = shares / a.kv_heads > 1 ? shares / a.kv_heads : 1;  // parts of a head
   int lo = (all + room - 1) / room, hi = most;
   lo = lo < S::LEAST ? S::LEAST : lo;
   hi = hi > lo ? hi : lo;
@@ -1061,31 +1061,35 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
     if (sum_of(n) <= room) hi = mid;
     else lo = mid + 1;
   }
-  int cut[PER], mine = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) mine += cut[j] = (steps[j] + lo - 1) / lo;
-  int x = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) red[wave] = x;
-  __syncthreads();
-  x -= mine;
-  for (int w = 0; w < wave; ++w) x += red[w];
+  int cut[PER], before[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const int i = PER * (int)threadIdx.x + j;
-    if (i <= slots) pre[i] = x;
-    x += cut[j];
+    int x = cut[j] = (steps[j] + lo - 1) / lo;
+    if (256 * j < slots)
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+      }
+    before[j] = x - cut[j];
+    if (lane == 63) red[8 + 4 * j + wave] = x;
   }
-  if (threadIdx.x == 255 && slots == S::MOST) pre[slots] = x;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    for (int w = 0; w < 4; ++w) {
+      if (w == wave) before[j] += sum;
+      sum += red[8 + 4 * j + w];
+    }
+    const int i = 256 * j + (int)threadIdx.x;
+    if (i < slots) pre[i] = before[j];
+    if (i == slots - 1) pre[slots] = before[j] + cut[j];
+  }
   __syncthreads();
   auto ahead = [&](int i) __attribute__((always_inline)) { return seq_same(pre[i]); };
   const int each = ahead(slots), parts_all = each * a.kv_heads;
-  // ---- this workgroup's part: those of an XCD side by side, as their keys are
+  // ---- this workgroup's part, those of an XCD side by side, as their keys are
   const int side = (parts_all + 7) / 8, part = block % 8 * side + block / 8;
   if (block / 8 >= side || part >= parts_all) return;
   const int head = part / each, r = part - head * each;
@@ -1107,7 +1111,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   st.load_q(a.q + (s.sp.first + s.token) * a.q_token + s.h * a.q_head, lane >> 5, a.kchunks);
   st.clear();
   const int n = s.t_hi > s.t_lo ? s.t_hi - s.t_lo : 0;
-  __syncthreads();  // the sums in the ring are read
+  __syncthreads();
   auto border = [&](int i) __attribute__((always_inline)) { return s.t_lo + (int)((int64_t)n * i / parts); };
   seq_tile_run<T, DP, true>(a, s, st, border(p), border(p + 1), lds0, tab, flag + 1, wave, lane);
   __syncthreads();
@@ -1150,8 +1154,10 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
 }
 
-// Sequences of many rows and of few at once: workgroups for the tiles of the one, behind them those for the keys of the other.  At heads
-// of 256 each fills the registers, and they are launches of their own.
+// Sequences of many rows and of few at once: half as many workgroups as the chip holds for the keys of the few between the first half
+// for parts of tiles and the rest of those, so that both kinds are there from the start.  Two portions of a prompt among 30 single
+// tokens, 32 heads of 64 over 4: 26 us (the portions alone 23, the single tokens alone 18), 34.5 with all for tiles ahead of as many
+// for the few.  At heads of 256 each kind fills the registers, and they are launches of their own.
 template <class T, int DP>
 struct SeqMixed {
   static constexpr int LDS = SeqTiles<T, DP>::LDS_SHARES > SeqRows<T, DP>::LDS ? SeqTiles<T, DP>::LDS_SHARES : SeqRows<T, DP>::LDS;
@@ -1160,12 +1166,14 @@ struct SeqMixed {
 template <class T, int DP>
 __global__ __launch_bounds__(256, (SeqMixed<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_mixed(const SeqRowsArgs a, int slots) {
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  if ((int)blockIdx.x < a.shares) seq_tile_shares<T, DP>(a, slots, blockIdx.x, smem_raw);
-  else seq_rows<T, DP>(a, (int)blockIdx.x - a.shares, smem_raw);
+  constexpr int N = SeqMixed<T, DP>::SHARES, H = N / 2;
+  const int i = blockIdx.x;
+  if (i < H || i >= 2 * H) seq_tile_shares<T, DP>(a, slots, N, i < H ? i : i - H, smem_raw);
+  else seq_rows<T, DP>(a, H, i - H, smem_raw);
 }
 template <class T, int DP>
 __global__ __launch_bounds__(256, 1) void k_seq_tile_shares(const SeqRowsArgs a, int slots) {
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  seq_tile_shares<T, DP>(a, slots, blockIdx.x, smem_raw);
+  seq_tile_shares<T, DP>(a, slots, SeqMixed<T, DP>::SHARES, blockIdx.x, smem_raw);
 }
 }  // namespace khm

@@ -68,25 +68,24 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   const SeqKv& kv = a.s.kv;
   auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 24; };  // 64 rows apart in 32 bits
   a.s.kv.plain = a.s.kchunks == CB && a.s.vchunks == CB && near(kv.k_slot) && near(kv.v_slot) && (!kv.pages || kv.page_size % (64 / CB) == 0);
-  a.shares = R::SHARES;
   a.all = how == FEW;
   if (how == FEW) return launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
   const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
   const dim3 grid((unsigned)(slots * a.s.kv_heads));
   if (how == PACKED) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
   // Tiles that are fewer than the workgroups the chip holds are cut along their keys (136 tiles of 512 tokens behind 16384 keys: 345 us,
-  // 1214 whole; 16 of 64 behind 4096: 33, 81); as many or more are left whole (520 of 2048 tokens behind 8192: 290 us, 333 with
-  // cuts).
-  if (slots <= S::MOST && slots * a.s.kv_heads <= M::SHARES) {
-    a.shares = M::SHARES;
+  // 1214 whole; 16 of 64 behind 4096: 33, 81); as many or more are left whole (512 of 2048 tokens behind 8192: 290 us, 333 with
+  // cuts).  How many there are depends on the offsets: by the tokens no more than these and one for each sequence.
+  unsigned parts = 0;
+  if (slots <= S::MOST && (int64_t)a.s.n_tokens * a.s.group / S::BM * a.s.kv_heads < M::SHARES) {
+    parts = ((unsigned)(slots * a.s.kv_heads > M::SHARES ? slots * a.s.kv_heads : M::SHARES) + 7) / 8 * 8;
     a.brought_tiles = a.brought + SEQ_SHARES;
     a.ws_tiles = a.ws + (size_t)2 * SEQ_SHARES * 32 * (a.s.vchunks * (16 / (int)sizeof(T)) + 4);
-    if constexpr (DP <= 128) return launch(k_seq_mixed<T, DP>, dim3(2 * M::SHARES), M::LDS, s, a, (int)slots);
+    if constexpr (DP <= 128) return launch(k_seq_mixed<T, DP>, dim3(M::SHARES / 2 + parts), M::LDS, s, a, (int)slots);
   }
   int rc;
-  if (DP > 128 && a.ws_tiles) rc = launch(k_seq_tile_shares<T, 256>, dim3(M::SHARES), S::LDS_SHARES, s, a, (int)slots);
+  if (DP > 128 && a.ws_tiles) rc = launch(k_seq_tile_shares<T, 256>, dim3(parts), S::LDS_SHARES, s, a, (int)slots);
   else rc = launch(k_seq_tiles<T, DP, true>, grid, S::LDS_PAGED, s, a.s);
-  a.shares = R::SHARES;
   return rc != KH_OK ? rc : launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
 }
 

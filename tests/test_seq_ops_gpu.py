@@ -426,7 +426,8 @@ def test_a_layer_s_attention_in_portions(gpu, dtype):
 CUT = [  # heads, kv_heads, key size, value size, new tokens, lengths, page: single tokens dealt by steps of keys, portions cut into parts
     (8, 1, 64, 64, [1], [20000], 16), (4, 1, 128, 128, [2, 1], [9000, 5], 16), (2, 1, 256, 256, [1], [3000], 32), (4, 2, 48, 80, [1, 3], [2500, 1], 8),
     (8, 1, 64, 64, [200], [6000], 3), (4, 2, 128, 128, [300, 1], [4000, 2000], 16), (4, 1, 256, 256, [60, 40, 1], [1500, 2100, 700], 32),
-    (8, 2, 128, 96, [257], [1700], 24)]
+    (8, 2, 128, 96, [257], [1700], 24),
+    (8, 8, 64, 64, [33] * 70 + [1] * 3, [90] * 70 + [1, 200, 3000], 16), (6, 6, 16, 256, [40] * 101, [57] * 101, 8)]  # more tiles than workgroups
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
