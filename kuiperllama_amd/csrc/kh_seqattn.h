@@ -64,9 +64,6 @@ struct SeqArgs {
   float c;                                                                 // scale log2(e)
 };
 
-// 16 bytes of zeros, for the chunks of a tile behind the end of its rows
-__device__ const f32x4 seq_zeros = {0.f, 0.f, 0.f, 0.f};
-
 // One sequence, with what the device's own numbers may not do to memory cut off.
 struct SeqSpan {
   int first, n, length;  // tokens [first, first + n), keys
@@ -85,12 +82,15 @@ __device__ __forceinline__ SeqSpan seq_span(const SeqArgs& a, int b) {
   return s;
 }
 
+// DP: elements of a row that are worked on, those behind a head's zeros in the queries and left out of the output.  A staged row has room
+// for 64, 128 or 256; behind the head's own lies its last chunk again.  (What it holds meets zeros; where that gives what is no
+// number, the row is done once more with care, as for any other.)
 template <class T, int DP>
 struct SeqCfg {
   static constexpr int E = 16 / (int)sizeof(T);
-  static constexpr int RB = DP * (int)sizeof(T);  // bytes of a staged row
+  static constexpr int RB = (DP <= 64 ? 64 : (DP <= 128 ? 128 : 256)) * (int)sizeof(T);  // bytes of a staged row
   static constexpr int CB = RB / 16;              // its chunks
-  static constexpr int NKB = RB / 32;             // its 32-byte k-blocks
+  static constexpr int NKB = DP * (int)sizeof(T) / 32;  // 32-byte k-blocks
   static constexpr int NMB = DP / 32;             // 32-column blocks of the output
   static constexpr bool TIGHT = RB > 256;         // queries and outputs fill the registers: reads of LDS stay near their use
   static constexpr bool HOLD = RB <= 512;         // queries in registers; else read again for each tile, under 128 products of 64 cycles
@@ -247,6 +247,8 @@ __device__ __forceinline__ void dma_x4_from(const char* addr, unsigned dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(addr), "s"(dst) : "memory", "m0");
 }
 #pragma clang diagnostic pop
+
+__device__ __forceinline__ int seq_chunk(int c, int chunks) { return c < chunks ? c : chunks - 1; }
 
 // Keys [lo, hi) of a sequence are those that anyone of a workgroup's rows sees: no other row, and no other page, is touched.
 struct SeqKeys {
@@ -452,8 +454,8 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
             v += place * a.kv.v_slot;
           }
           const unsigned at = (unsigned)((S::W * j + wave) * 1024);
-          dma_x4_keep(k, (unsigned)(r * (int)a.kv.k_slot + 16 * (c ^ C::turn_k(row + r))), K + at);
-          dma_x4_keep(v, (unsigned)(r * (int)a.kv.v_slot + 16 * (c ^ C::turn_v(row + r))), V + at);
+          dma_x4_keep(k, (unsigned)(r * (int)a.kv.k_slot + 16 * seq_chunk(c ^ C::turn_k(row + r), a.kchunks)), K + at);
+          dma_x4_keep(v, (unsigned)(r * (int)a.kv.v_slot + 16 * seq_chunk(c ^ C::turn_v(row + r), a.vchunks)), V + at);
         }
         return;
       }
@@ -472,8 +474,8 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
           vo = place * a.kv.v_slot;
         }
         const unsigned at = (unsigned)((S::W * j + wave) * 1024);
-        dma_x4_from(ck < a.kchunks ? s.x.k + ko + 16 * ck : (const char*)&seq_zeros, K + at);
-        dma_x4_from(cv < a.vchunks ? s.x.v + vo + 16 * cv : (const char*)&seq_zeros, V + at);
+        dma_x4_from(s.x.k + ko + 16 * seq_chunk(ck, a.kchunks), K + at);
+        dma_x4_from(s.x.v + vo + 16 * seq_chunk(cv, a.vchunks), V + at);
         if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -840,7 +842,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
           for (int j = 0; j < S::NL; ++j) {
             const int key = k0 + j * RPR, p = seq_page(a.kv, key), page = seq_same(tab[p - p0]);
             dma_x4_keep(base + page * ps + (key - p * a.kv.page_size) * ss,
-                        (unsigned)(r * (int)ss + 16 * (c ^ (keys ? C::turn_k(j * RPR + r) : C::turn_v(j * RPR + r)))), dst + 1024 * j);
+                        (unsigned)(r * (int)ss + 16 * seq_chunk(c ^ (keys ? C::turn_k(j * RPR + r) : C::turn_v(j * RPR + r)), chunks)), dst + 1024 * j);
           }
           return;
         }
@@ -850,7 +852,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
           int key = k0 + r;
           key = key < ka ? ka : (key >= kb ? kb - 1 : key);
           const int p = seq_page(a.kv, key), sl = key - p * a.kv.page_size, page = tab[p - p0];
-          dma_x4_from(c < chunks ? base + page * ps + sl * ss + 16 * c : (const char*)&seq_zeros, dst + 1024 * j);
+          dma_x4_from(base + page * ps + sl * ss + 16 * seq_chunk(c, chunks), dst + 1024 * j);
           if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
       };
@@ -1115,7 +1117,7 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   auto border = [&](int i) __attribute__((always_inline)) { return s.t_lo + (int)((int64_t)n * i / parts); };
   seq_tile_run<T, DP, true>(a, s, st, border(p), border(p + 1), lds0, tab, flag + 1, wave, lane);
   __syncthreads();
-  float l = flag[1] ? NAN : xor32_sum(st.l);
+  float l = flag[1] ? -1.f : xor32_sum(st.l);  // -1: of a page that is none
   if (parts > 1) {
     const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64, first = part - p;  // pitch of a wave
     auto at = [&](int i) __attribute__((always_inline)) { return ra.ws_tiles + (size_t)(first + i) * 4 * pitch + wave * pitch + lane; };
@@ -1138,20 +1140,23 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
     float m = -INFINITY;
     for (int i = 0; i < parts; ++i) m = fmaxf(m, seq_take(at(i) + (16 * blocks) * 64));
     st.clear();
+    bool none = false;
     l = 0.f;
     for (int i = 0; i < parts; ++i) {
       const float* from = at(i);
       const float mp = seq_take(from + (16 * blocks) * 64), lp = seq_take(from + (16 * blocks + 1) * 64);
       const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
-      l += mp == -INFINITY ? lp : lp * f;  // NaN of a page that is none
+      none |= lp < 0.f;
+      l += lp * f;
 #pragma unroll
       for (int n = 0; n < C::NMB; ++n)
         if (n < blocks)
 #pragma unroll
           for (int j = 0; j < 16; ++j) st.o[n][j] = __builtin_fmaf(seq_take(from + (16 * n + j) * 64), f, st.o[n][j]);
     }
+    if (none) l = -1.f;
   }
-  seq_tile_write<T, DP, true>(a, s, st, l, !(l == l), lane);
+  seq_tile_write<T, DP, true>(a, s, st, l, l < 0.f, lane);
 }
 
 // Sequences of many rows and of few at once: half as many workgroups as the chip holds for the keys of the few between the first half

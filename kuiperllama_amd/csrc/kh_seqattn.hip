@@ -67,7 +67,7 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   constexpr int CB = SeqCfg<T, DP>::CB;
   const SeqKv& kv = a.s.kv;
   auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 24; };  // 64 rows apart in 32 bits
-  a.s.kv.plain = a.s.kchunks == CB && a.s.vchunks == CB && near(kv.k_slot) && near(kv.v_slot) && (!kv.pages || kv.page_size % (64 / CB) == 0);
+  a.s.kv.plain = near(kv.k_slot) && near(kv.v_slot) && (!kv.pages || kv.page_size % (64 / CB) == 0);
   a.all = how == FEW;
   if (how == FEW) return launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
   const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
@@ -91,8 +91,8 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
 
 int go(const SeqRowsArgs& a, int e, How how, hipStream_t s) {
   const int most = (a.s.kchunks > a.s.vchunks ? a.s.kchunks : a.s.vchunks) * 16 / e;
-  if (e == 2) return most <= 64 ? go<bf16, 64>(a, how, s) : (most <= 128 ? go<bf16, 128>(a, how, s) : go<bf16, 256>(a, how, s));
-  return most <= 64 ? go<float, 64>(a, how, s) : (most <= 128 ? go<float, 128>(a, how, s) : go<float, 256>(a, how, s));
+  if (e == 2) return most <= 64 ? go<bf16, 64>(a, how, s) : most <= 96 ? go<bf16, 96>(a, how, s) : (most <= 128 ? go<bf16, 128>(a, how, s) : go<bf16, 256>(a, how, s));
+  return most <= 64 ? go<float, 64>(a, how, s) : most <= 96 ? go<float, 96>(a, how, s) : (most <= 128 ? go<float, 128>(a, how, s) : go<float, 256>(a, how, s));
 }
 }  // namespace
 }  // namespace khm
