@@ -660,13 +660,13 @@ struct SeqRows {
 };
 
 // The final rows of a unit: o / l, and with care where that is no number.
-template <class T>
+template <class T, bool PAGED>
 __device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, int b, int head, int r0, int rows, bool odd, int wave, int lane) {
   if (!odd) return;
   for (int r = r0 + wave; r < r0 + rows; r += 4) {
     const int tk = r / a.group, h = head * a.group + r - tk * a.group, place = u.sp.length - u.sp.n + tk;
     SeqKeys x = seq_keys(a, b, head, u.sp, place, place);
-    seq_one<T, true>(a, x, a.q + (u.sp.first + tk) * a.q_token + h * a.q_head, a.out + (u.sp.first + tk) * a.o_token + h * a.o_head, place, lane);
+    seq_one<T, PAGED>(a, x, a.q + (u.sp.first + tk) * a.q_token + h * a.q_head, a.out + (u.sp.first + tk) * a.o_token + h * a.o_head, place, lane);
   }
 }
 
@@ -758,8 +758,8 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
   return odd;
 }
 
-// Workgroup `share` of `shares`
-template <class T, int DP>
+// Workgroup `share` of `shares`; whole prompts: 32 rows of a key head, slot of 32 rows by slot
+template <class T, int DP, bool PAGED>
 __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int share, char* smem_raw) {
   typedef SeqRows<T, DP> S;
   typedef SeqCfg<T, DP> C;
@@ -772,38 +772,65 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
   const unsigned ring = lds0 + (unsigned)(wave * S::NB * S::TB);
   // ---- this workgroup's share
-  const SeqScan sc = seq_scan(ra, red);
-  const int n_shares = seq_shares(sc.total, shares);
-  if (share >= n_shares) return;
-  int64_t at = seq_share(sc.total, n_shares, share);
-  const int64_t end = seq_share(sc.total, n_shares, share + 1);
-  if (sc.before <= at && at < sc.before + sc.mine) {  // one thread
-    int64_t p = sc.before;
-    int b = (int)threadIdx.x * sc.per;
-    for (;; ++b) {
-      const int64_t n = seq_units(ra, b).all;
-      if (at < p + n) break;
-      p += n;
+  SeqScan sc;
+  SeqUnits u;
+  int n_shares = 1, b = 0, head = 0, r0 = 0, ta = 0, tb = 0, places = 0, unit = 0;
+  int64_t at = 0, end = 1, ahead = 0;  // ahead: places ahead of sequence b
+  if constexpr (PAGED) {
+    sc = seq_scan(ra, red);
+    n_shares = seq_shares(sc.total, shares);
+    if (share >= n_shares) return;
+    at = seq_share(sc.total, n_shares, share);
+    end = seq_share(sc.total, n_shares, share + 1);
+    if (sc.before <= at && at < sc.before + sc.mine) {  // one thread
+      int64_t p = sc.before;
+      int b = (int)threadIdx.x * sc.per;
+      for (;; ++b) {
+        const int64_t n = seq_units(ra, b).all;
+        if (at < p + n) break;
+        p += n;
+      }
+      flag[0] = b;
+      *(int64_t*)(flag + 2) = p;
     }
-    flag[0] = b;
-    *(int64_t*)(flag + 2) = p;
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(flag[0]);
+    ahead = *(int64_t*)(flag + 2);
+    u = seq_units(ra, b);
+  } else {
+    const int slot = share / a.kv_heads;
+    b = seq_same(seq_of_slot(a, slot, 32, lane));
+    u.sp = seq_span(a, b);
+    u.rows = u.sp.n * a.group;
+    u.blocks = (u.rows + 31) / 32;
+    head = share - slot * a.kv_heads;
+    r0 = 32 * (u.blocks - 1 - (slot - seq_slot_base(a, b, 32)));  // long ones first
+    if (r0 < 0 || r0 >= u.rows) return;
+    const int first = r0 / a.group, last = (r0 + 31 < u.rows ? r0 + 31 : u.rows - 1) / a.group;
+    u.lo = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
+    u.hi = last + 1;
+    u.t0 = u.lo / SEQ_STEP;
+    tb = u.steps = (u.hi + SEQ_STEP - 1) / SEQ_STEP - u.t0;
   }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(flag[0]);
-  int64_t ahead = *(int64_t*)(flag + 2);  // places ahead of sequence b
-  SeqUnits u = seq_units(ra, b);
   int p0 = 0, tab_b = -1, tab_ka = 0, tab_kb = 0;  // the table holds the pages of keys [tab_ka, tab_kb) of tab_b, from page p0 on
   while (at < end) {
-    while (at >= ahead + u.all) {
-      ahead += u.all;
-      u = seq_units(ra, ++b);
+    if constexpr (PAGED) {
+      while (at >= ahead + u.all) {
+        ahead += u.all;
+        u = seq_units(ra, ++b);
+      }
+      places = u.steps + SEQ_HEAD;
+      unit = (int)((at - ahead) / places);
+      const int from = (int)((at - ahead) - (int64_t)unit * places), to = places - from < end - at ? places : from + (int)(end - at);
+      at += to - from;
+      ta = from > SEQ_HEAD ? from - SEQ_HEAD : 0;
+      tb = to > SEQ_HEAD ? to - SEQ_HEAD : 0;
+      if (tb <= ta) continue;  // nothing but the unit's head: the workgroup that follows begins it
+      head = unit / u.blocks;
+      r0 = 32 * (unit - head * u.blocks);
+    } else {
+      at = end;
     }
-    const int places = u.steps + SEQ_HEAD, unit = (int)((at - ahead) / places), from = (int)((at - ahead) - (int64_t)unit * places);
-    const int to = places - from < end - at ? places : from + (int)(end - at);
-    at += to - from;
-    const int ta = from > SEQ_HEAD ? from - SEQ_HEAD : 0, tb = to > SEQ_HEAD ? to - SEQ_HEAD : 0;
-    if (tb <= ta) continue;  // nothing but the unit's head: the workgroup that follows begins it
-    const int head = unit / u.blocks, r0 = 32 * (unit - head * u.blocks);
     const int n_rows = u.rows - r0 < 32 ? u.rows - r0 : 32;
     const int row = r0 + ((lane & 31) < n_rows ? (lane & 31) : n_rows - 1);
     const int token = row / a.group, h = head * a.group + row - token * a.group, place = u.sp.length - u.sp.n + token;
@@ -813,13 +840,13 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
     SeqState<T, DP> st;
     st.load_q(a.q + (u.sp.first + token) * a.q_token + h * a.q_head, half, a.kchunks);
     st.clear();
-    if (threadIdx.x == 0 && b != tab_b) flag[1] = x.bad;  // and stays set for the sequence: nothing of it is a number then
-    const int per_table = seq_table_steps(a.kv, SEQ_STEP);
+    if (PAGED && threadIdx.x == 0 && b != tab_b) flag[1] = x.bad;  // and stays set for the sequence: nothing of it is a number then
+    const int per_table = PAGED ? seq_table_steps(a.kv, SEQ_STEP) : tb - ta;
     for (int c0 = ta; c0 < tb && u.hi > u.lo; c0 += per_table) {
       const int c1 = tb - c0 < per_table ? tb : c0 + per_table;
       const int ka = (u.t0 + c0) * SEQ_STEP > u.lo ? (u.t0 + c0) * SEQ_STEP : u.lo, kb = (u.t0 + c1) * SEQ_STEP < u.hi ? (u.t0 + c1) * SEQ_STEP : u.hi;
       __syncthreads();  // the table before, and partial outputs, are read
-      if (b != tab_b || ka != tab_ka || kb > tab_kb) {  // not that of the key head before
+      if (PAGED && (b != tab_b || ka != tab_ka || kb > tab_kb)) {  // not that of the key head before
         p0 = seq_table(a.kv, x.table, ka, kb, tab, flag + 1);
         tab_b = b;
         tab_ka = ka;
@@ -840,9 +867,13 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
           const int r = seq_fresh<C::TIGHT>(lane) / C::CB, c = lane % C::CB;
 #pragma unroll
           for (int j = 0; j < S::NL; ++j) {
-            const int key = k0 + j * RPR, p = seq_page(a.kv, key), page = seq_same(tab[p - p0]);
-            dma_x4_keep(base + page * ps + (key - p * a.kv.page_size) * ss,
-                        (unsigned)(r * (int)ss + 16 * seq_chunk(c ^ (keys ? C::turn_k(j * RPR + r) : C::turn_v(j * RPR + r)), chunks)), dst + 1024 * j);
+            const int key = k0 + j * RPR;
+            int64_t at = key * ss;
+            if constexpr (PAGED) {
+              const int p = seq_page(a.kv, key), page = seq_same(tab[p - p0]);
+              at = page * ps + (key - p * a.kv.page_size) * ss;
+            }
+            dma_x4_keep(base + at, (unsigned)(r * (int)ss + 16 * seq_chunk(c ^ (keys ? C::turn_k(j * RPR + r) : C::turn_v(j * RPR + r)), chunks)), dst + 1024 * j);
           }
           return;
         }
@@ -851,8 +882,12 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
           const int i = j * 64 + seq_fresh<(C::RB > 128)>(lane), r = i / C::CB, c = (i - r * C::CB) ^ (keys ? C::turn_k(r) : C::turn_v(r));
           int key = k0 + r;
           key = key < ka ? ka : (key >= kb ? kb - 1 : key);
-          const int p = seq_page(a.kv, key), sl = key - p * a.kv.page_size, page = tab[p - p0];
-          dma_x4_from(base + page * ps + sl * ss + 16 * seq_chunk(c, chunks), dst + 1024 * j);
+          int64_t at = key * ss;
+          if constexpr (PAGED) {
+            const int p = seq_page(a.kv, key);
+            at = tab[p - p0] * ps + (key - p * a.kv.page_size) * ss;
+          }
+          dma_x4_from(base + at + 16 * seq_chunk(c, chunks), dst + 1024 * j);
           if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
       };
@@ -921,10 +956,10 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
         }
     }
     __syncthreads();
-    const bool bad = flag[1] != 0;
+    const bool bad = PAGED && flag[1] != 0;
     const int cols = a.vchunks * C::E;
-    const bool whole = ta == 0 && tb == u.steps;
-    float* ws = ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4);
+    const bool whole = !PAGED || (ta == 0 && tb == u.steps);
+    float* ws = PAGED ? ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4) : nullptr;
     bool odd = false;
     for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
       const int r = e / cols, d = e - r * cols;
@@ -951,7 +986,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
         }
       }
     }
-    if (!whole) {
+    if (PAGED && !whole) {
       int i0;
       const int parts = seq_parts(sc.total, n_shares, ahead + (int64_t)unit * places, places, i0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
@@ -969,7 +1004,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
     if (lane == 0) flag[4 + wave] = any;
     __syncthreads();
     odd = flag[4] | flag[5] | flag[6] | flag[7];
-    seq_finish<T>(a, u, b, head, r0, n_rows, odd, wave, lane);
+    seq_finish<T, PAGED>(a, u, b, head, r0, n_rows, odd, wave, lane);
   }
 }
 
@@ -977,7 +1012,14 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
 template <class T, int DP>
 __global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_rows(const SeqRowsArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  seq_rows<T, DP>(a, SeqRows<T, DP>::SHARES, blockIdx.x, smem_raw);
+  seq_rows<T, DP, true>(a, SeqRows<T, DP>::SHARES, blockIdx.x, smem_raw);
+}
+
+// Whole prompts that are few tiles of 128 rows: 32 rows a workgroup, and a quarter of their keys a wave.  grid (slots * kv_heads)
+template <class T, int DP>
+__global__ __launch_bounds__(256, (SeqRows<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) void k_seq_blocks(const SeqArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  seq_rows<T, DP, false>(SeqRowsArgs{a}, 0, blockIdx.x, smem_raw);
 }
 
 // ---- many rows, few tiles ----------------------------------------------------------------------------------------------------------
@@ -1174,7 +1216,7 @@ __global__ __launch_bounds__(256, (SeqMixed<T, DP>::LDS <= 80 * 1024 ? 2 : 1)) v
   constexpr int N = SeqMixed<T, DP>::SHARES, H = N / 2;
   const int i = blockIdx.x;
   if (i < H || i >= 2 * H) seq_tile_shares<T, DP>(a, slots, N, i < H ? i : i - H, smem_raw);
-  else seq_rows<T, DP>(a, H, i - H, smem_raw);
+  else seq_rows<T, DP, true>(a, H, i - H, smem_raw);
 }
 template <class T, int DP>
 __global__ __launch_bounds__(256, 1) void k_seq_tile_shares(const SeqRowsArgs a, int slots) {

@@ -56,7 +56,7 @@ int launch(K kern, dim3 grid, int lds, hipStream_t s, const A&... a) {
   return kh_launch_status();
 }
 
-// How a call is launched: TILES alone (whole prompts), or over pages - ROWS alone where no sequence has more than 32 of them, else tiles
+// How a call is launched: whole prompts in tiles of 128 rows or of 32, or over pages - ROWS alone where no sequence has more than 32 of them, else tiles
 // of rows and, at once or behind them, the rows of the sequences that have few.
 enum How { PACKED, FEW, ANY };
 template <class T, int DP>
@@ -72,7 +72,18 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   if (how == FEW) return launch(k_seq_rows<T, DP>, dim3(R::SHARES), R::LDS, s, a);
   const int64_t slots = (int64_t)a.s.n_tokens * a.s.group / S::BM + a.s.n_seqs;
   const dim3 grid((unsigned)(slots * a.s.kv_heads));
-  if (how == PACKED) return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
+  if (how == PACKED) {
+    // Tiles that are too few wait for the longest of them, which workgroups of 32 rows and a quarter of the keys a wave have done in a fourth
+    // of the time, for four times the requests.  us, blocks and tiles of 128: bf16 heads of 128, 14 over 2, 1000 tokens (109 tiles) 20, 29;
+    // 32 over 8, 1024 (256) 37, 33; 250 of 14 over 2: 11.6, 11.0.  fp32, 14 over 2, 1000 tokens 64, 145; 32 over 8, 1024: 137, 150; 2048
+    // (512) 440, 383; 8 x 64 of 32 over 32: 32, 24.
+    const bool fp32 = sizeof(T) == 4;
+    if ((int64_t)a.s.n_tokens * a.s.group / S::BM * a.s.kv_heads < (fp32 ? 512 : 256) && a.s.n_tokens / a.s.n_seqs >= (fp32 ? 192 : 384)) {
+      const int64_t blocks = (int64_t)a.s.n_tokens * a.s.group / 32 + a.s.n_seqs;
+      return launch(k_seq_blocks<T, DP>, dim3((unsigned)(blocks * a.s.kv_heads)), R::LDS, s, a.s);
+    }
+    return launch(k_seq_tiles<T, DP, false>, grid, S::LDS_PACKED, s, a.s);
+  }
   // Tiles that are fewer than the workgroups the chip holds are cut along their keys (136 tiles of 512 tokens behind 16384 keys: 345 us,
   // 1214 whole; 16 of 64 behind 4096: 33, 81); as many or more are left whole (512 of 2048 tokens behind 8192: 290 us, 333 with
   // cuts).  How many there are depends on the offsets: by the tokens no more than these and one for each sequence.

@@ -156,7 +156,9 @@ def offsets_of(lens, device):
 PACKED = [  # heads, kv_heads, key size, value size, lengths, window
     (14, 2, 64, 64, [7, 33, 1], 0), (32, 8, 64, 64, [300, 0, 128, 129, 1, 64], 0), (4, 4, 128, 128, [513], 0), (6, 6, 48, 48, [31, 32, 33, 65], 0),
     (12, 1, 128, 128, [100, 11], 0), (8, 2, 64, 64, [500, 20], 100), (8, 8, 64, 64, [200], 1), (3, 1, 80, 40, [150, 3], 64), (5, 5, 16, 256, [130], 0),
-    (4, 2, 256, 256, [140, 70], 37), (7, 1, 192, 128, [90], 0), (2, 1, 8, 8, [40, 1, 1], 0), (1, 1, 64, 64, [1030], 129), (64, 1, 64, 64, [9, 2], 0)]
+    (4, 2, 256, 256, [140, 70], 37), (7, 1, 192, 128, [90], 0), (2, 1, 8, 8, [40, 1, 1], 0), (1, 1, 64, 64, [1030], 129), (64, 1, 64, 64, [9, 2], 0),
+    # few tiles, long prompts: blocks of 32 rows
+    (14, 2, 64, 64, [700], 0), (12, 1, 128, 128, [400, 0, 1000], 150), (3, 3, 96, 96, [1000, 385], 0), (2, 1, 256, 192, [500], 0), (5, 1, 40, 72, [901], 300)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
@@ -184,18 +186,19 @@ def test_packed(gpu, dtype, case):
         close(out[:T], *attended(q[:T], k[:T], v[:T], 0, 0.5), "scale")
 
 
+@pytest.mark.parametrize("n", [150, 900], ids=["tiles", "blocks"])
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
-def test_what_a_query_does_not_see_does_not_reach_it(gpu, dtype):
+def test_what_a_query_does_not_see_does_not_reach_it(gpu, dtype, n):
     """Infinities and NaN in keys and values of later tokens, and of tokens before the window."""
     from kuiperllama_amd import ops
     gen = generator(3)
-    H, KH, D, n, window = 4, 2, 64, 150, 20
+    H, KH, D, window = 4, 2, 64, 20
     q, k, v = rnd(gen, dtype, n, H, D), rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, D)
     want, bound = attended(q, k, v, window, D ** -0.5)
     for t, value in ((40, math.inf), (41, math.nan), (75, -math.inf)):
         v[t, :, t % 7::5] = value
     k[100] = math.nan
-    k[149, 1, 3] = math.inf
+    k[n - 1, 1, 3] = math.inf
     out = torch.empty(n, H, D, dtype=dtype, device=gpu)
     ops.attn_packed(q, k, v, offsets_of([n], gpu), out, window=window)
     rows = torch.arange(n, device=gpu)
@@ -203,7 +206,7 @@ def test_what_a_query_does_not_see_does_not_reach_it(gpu, dtype):
     for t in (40, 41, 75):
         hit[(rows >= t) & (rows < t + window), :, t % 7::5] = True
     hit[(rows >= 100) & (rows < 100 + window)] = True
-    hit[149, 2:] = True
+    hit[n - 1, 2:] = True
     close(out[~hit], want[~hit], bound[~hit])
     assert not torch.isfinite(out[rows < 100][hit[rows < 100]]).any()
     at40 = out[40, :, 40 % 7::5]
