@@ -18,6 +18,8 @@
 #pragma once
 #include "kh_lgemm.h"
 
+#include <type_traits>
+
 namespace khm {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -35,12 +37,37 @@ struct Tile32<bf16> {
 template <>
 struct Tile32<float> {
   typedef f32x4 frag;
-  static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, f32x16 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  }
 };
+
+// fp32 on the bf16 matrix cores: a number is the sum of three of 8 bits, exactly - rounded to bf16, what is left rounded, what is left then.
+// Of the nine products of two numbers the three smallest are left out, at most 2^-24 of the product each and of either sign: less than the
+// fp32 matrix instruction's own rounding of n sums, for 6 x 32 cycles a block of 16 and not 8 x 64.
+struct Split {
+  bf16x8 h, m, l;
+};
+__device__ __forceinline__ Split seq_split(const float (&x)[8]) {
+  Split s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    s.h[i] = (bf16)x[i];
+    const float r = x[i] - (float)s.h[i];
+    s.m[i] = (bf16)r;
+    s.l[i] = (bf16)(r - (float)s.m[i]);
+  }
+  return s;
+}
+__device__ __forceinline__ Split seq_split(const f32x4& a, const f32x4& b) {
+  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  return seq_split(x);
+}
+// the products but the largest
+__device__ __forceinline__ f32x16 mma_small(const Split& a, const Split& b, f32x16 c) {
+  c = Tile32<bf16>::mma(a.l, b.h, c);
+  c = Tile32<bf16>::mma(a.h, b.l, c);
+  c = Tile32<bf16>::mma(a.m, b.m, c);
+  c = Tile32<bf16>::mma(a.m, b.h, c);
+  return Tile32<bf16>::mma(a.h, b.m, c);
+}
 
 // Where keys and values are.  Strides in bytes.
 struct SeqKv {
@@ -92,7 +119,7 @@ struct SeqCfg {
   static constexpr int CB = RB / 16;              // its chunks
   static constexpr int NKB = DP * (int)sizeof(T) / 32;  // 32-byte k-blocks
   static constexpr int NMB = DP / 32;             // 32-column blocks of the output
-  static constexpr bool TIGHT = RB > 256;         // queries and outputs fill the registers: reads of LDS stay near their use
+  static constexpr bool TIGHT = RB > 256 || sizeof(T) == 4;  // queries and outputs fill the registers: reads of LDS stay near their use
   static constexpr bool HOLD = RB <= 512;         // queries in registers; else read again for each tile, under 128 products of 64 cycles
   // LDS: chunk c of row r of the keys lies in slot c ^ turn_k(r), of the values in c ^ turn_v(r).  Reads of 16 bytes of 16 rows
   // (keys), of 32 bytes of four rows (values) then touch every bank once.  turn_v(r + 8) = turn_v(r), turn_v(4 + i) = turn_v(4) ^ turn_v(i),
@@ -125,7 +152,9 @@ template <class T, int DP>
 struct SeqState {
   typedef SeqCfg<T, DP> C;
   typedef typename Tile32<T>::frag frag;
-  frag q[C::HOLD ? C::NKB : 1];
+  // queries, by blocks of 32 bytes; fp32: by two of them
+  static constexpr int PER = sizeof(T) == 2 ? 1 : 2;
+  typename std::conditional<sizeof(T) == 2, frag, Split>::type q[C::HOLD ? C::NKB / PER : 1];
   const char* row;  // of the queries
   int chunks;
   f32x16 o[C::NMB];
@@ -153,7 +182,10 @@ struct SeqState {
     chunks = n;
     if constexpr (C::HOLD)
 #pragma unroll
-      for (int b = 0; b < C::NKB; ++b) q[b] = query(b, half);
+      for (int b = 0; b < C::NKB / PER; ++b) {
+        if constexpr (PER == 1) q[b] = query(b, half);
+        else q[b] = seq_split(query(2 * b, half), query(2 * b + 1, half));
+      }
   }
   // scores of 32 keys, rows r0 .. of the tile at K
   __device__ __forceinline__ f32x16 scores(unsigned K, int r0, int lane) const {
@@ -162,10 +194,24 @@ struct SeqState {
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
     const int r = lane & 31;
     const unsigned at = K + (unsigned)(r * C::RB + 16 * ((lane >> 5) ^ C::turn_k(r)));
+    if constexpr (PER == 1) {
 #pragma unroll
-    for (int b = 0; b < C::NKB; ++b) {
-      s = Tile32<T>::mma(lds_read<frag>((at ^ (32 * b)) + r0 * C::RB), C::HOLD ? q[C::HOLD ? b : 0] : query(b, lane >> 5), s);
-      if (C::TIGHT && b % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int b = 0; b < C::NKB; ++b) {
+        s = Tile32<T>::mma(lds_read<frag>((at ^ (32 * b)) + r0 * C::RB), q[b], s);
+        if (C::TIGHT && b % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      f32x16 small = s;  // apart: as many roundings of the sum as it has blocks
+#pragma unroll
+      for (int b = 0; b < C::NKB / 2; ++b) {
+        const Split k = seq_split(lds_read<frag>((at ^ (64 * b)) + r0 * C::RB), lds_read<frag>((at ^ (64 * b + 32)) + r0 * C::RB));
+        const Split& x = C::HOLD ? q[C::HOLD ? b : 0] : seq_split(query(2 * b, lane >> 5), query(2 * b + 1, lane >> 5));
+        small = mma_small(k, x, small);
+        s = Tile32<bf16>::mma(k.h, x.h, s);
+        if (b % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] += small[i];
     }
     return s;
   }
@@ -219,12 +265,21 @@ struct SeqState {
     } else {
       const unsigned at = V + (unsigned)(4 * half * C::RB + 16 * (((lane & 31) >> 2) ^ C::turn_v(4 * half)) + 4 * (lane & 3));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int t = 0; t < 2; ++t) {
+        float w[8];
 #pragma unroll
-        for (int n = 0; n < C::NMB; ++n)
-          o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(lds_read<float>((at ^ (16 * C::turn_v(i & 3) + 128 * n)) + (r0 + 8 * (i >> 2) + (i & 3)) * C::RB), p[i], o[n],
-                                                      0, 0, 0);
-        if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 8; ++j) w[j] = p[8 * t + j];
+        const Split x = seq_split(w);
+#pragma unroll
+        for (int n = 0; n < C::NMB; ++n) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            v[j] = lds_read<float>((at ^ (16 * C::turn_v(j & 3) + 128 * n)) + (r0 + 16 * t + 8 * (j >> 2) + (j & 3)) * C::RB);
+          const Split y = seq_split(v);
+          o[n] = Tile32<bf16>::mma(y.h, x.h, mma_small(y, x, o[n]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
@@ -544,7 +599,7 @@ __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, con
 // 64 (863 TFLOP/s), 585 at 128 (945), where the chip clocks down to 1.86 GHz and the matrix cores are busy 44 % of its cycles, the vector
 // unit (exponentials, maxima) 53.
 template <class T, int DP, bool PAGED>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : (DP <= 128 ? 2 : 1)) void k_seq_tiles(const SeqArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 3 : (DP <= 128 ? 2 : 1)) void k_seq_tiles(const SeqArgs a) {
   typedef SeqTiles<T, DP> S;
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   int *tab = (int*)(smem_raw + S::RING), *bad = tab + SEQ_TAB;
