@@ -56,8 +56,8 @@ int launch(K kern, dim3 grid, int lds, hipStream_t s, const A&... a) {
   return kh_launch_status();
 }
 
-// How a call is launched: whole prompts in tiles of 128 rows or of 32, or over pages - ROWS alone where no sequence has more than 32 of them, else tiles
-// of rows and, at once or behind them, the rows of the sequences that have few.
+// How a call is launched: whole prompts, in tiles of 128 rows or of 32; over pages, few rows alone where no sequence has more than 32, else
+// tiles of rows and, at once or behind them, the rows of the sequences that have few.
 enum How { PACKED, FEW, ANY };
 template <class T, int DP>
 int go(SeqRowsArgs a, How how, hipStream_t s) {
@@ -74,11 +74,12 @@ int go(SeqRowsArgs a, How how, hipStream_t s) {
   const dim3 grid((unsigned)(slots * a.s.kv_heads));
   if (how == PACKED) {
     // Tiles that are too few wait for the longest of them, which workgroups of 32 rows and a quarter of the keys a wave have done in a fourth
-    // of the time, for four times the requests.  us, blocks and tiles of 128: bf16 heads of 128, 14 over 2, 1000 tokens (109 tiles) 20, 29;
-    // 32 over 8, 1024 (256) 37, 33; 250 of 14 over 2: 11.6, 11.0.  fp32, 14 over 2, 1000 tokens 64, 145; 32 over 8, 1024: 137, 150; 2048
-    // (512) 440, 383; 8 x 64 of 32 over 32: 32, 24.
+    // of the time, for four times the requests.  us, blocks and tiles of 128: bf16, heads of 128, 14 over 2, 1000 tokens (109 tiles) 20, 29;
+    // 2000 (218) 46, 57; 32 over 8, 1024 (256) 37, 33; 250 of 14 over 2 12, 11.  fp32, 14 over 2, 1000 tokens 64, 130; 4000 (437) 625,
+    // 501, of 64 235, 286; 8 x 64 of 32 over 32 34, 22.
     const bool fp32 = sizeof(T) == 4;
-    if ((int64_t)a.s.n_tokens * a.s.group / S::BM * a.s.kv_heads < (fp32 ? 512 : 256) && a.s.n_tokens / a.s.n_seqs >= (fp32 ? 192 : 384)) {
+    const int most = fp32 ? (DP <= 64 ? 512 : 256) : 224;
+    if ((int64_t)a.s.n_tokens * a.s.group / S::BM * a.s.kv_heads <= most && a.s.n_tokens / a.s.n_seqs >= (fp32 ? 192 : 384)) {
       const int64_t blocks = (int64_t)a.s.n_tokens * a.s.group / 32 + a.s.n_seqs;
       return launch(k_seq_blocks<T, DP>, dim3((unsigned)(blocks * a.s.kv_heads)), R::LDS, s, a.s);
     }
