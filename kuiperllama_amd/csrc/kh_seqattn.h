@@ -725,12 +725,17 @@ __device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, 
   }
 }
 
-// Partial results pass between workgroups, maybe of different XCDs, in agent-scope words, which are stored through and read past the
-// caches that are not common: with 512 workgroups, a fence for each part costs the launch 15 - 20 us.
-__device__ __forceinline__ void seq_give(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float seq_take(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ f32x4 seq_take4(const float* p) {
-  return f32x4{seq_take(p), seq_take(p + 1), seq_take(p + 2), seq_take(p + 3)};
+// Partial results pass between workgroups, maybe of different XCDs, in words of agent scope, which are stored through and read past the
+// caches that are not common (a fence for each part instead costs a launch of 512 workgroups 15 - 20 us), four at a time: an atomic load
+// has one, and the joining workgroup waits for as many requests as it can have under way.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t seq_parts_at(float* p) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00020000); }
+constexpr int SEQ_AGENT = 16;  // sc1
+__device__ __forceinline__ void seq_give(__amdgpu_buffer_rsrc_t to, unsigned at, const f32x4& v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, (int)(4 * at), 0, SEQ_AGENT);
+}
+__device__ __forceinline__ f32x4 seq_take(__amdgpu_buffer_rsrc_t from, unsigned at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(4 * at), 0, SEQ_AGENT));
 }
 
 // The rows of a unit from its parts: their weights (LDS, as many rows at a time as fit `room` floats), then their outputs, four columns a
@@ -741,7 +746,8 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
   const SeqArgs& a = ra.s;
   const int cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 4;
   // part p: the end of workgroup i0's share for the first, the beginning of that of i0 + p for the others
-  auto at = [&](int r, int p) __attribute__((always_inline)) { return ra.ws + ((size_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * 32 + r) * pitch; };
+  auto at = [&](int r, int p) __attribute__((always_inline)) { return (unsigned)(((2 * (i0 + p) + (p == 0 ? 1 : 0)) * 32 + r) * pitch); };
+  const __amdgpu_buffer_rsrc_t ws = seq_parts_at(ra.ws);
   int across = 1, down = 1;  // threads of a row: its columns by four; rows at once
   while (across * 4 < cols) across *= 2;
   while (down < n_rows && down * across < 256 && 2 * down * parts <= room) down *= 2;
@@ -757,8 +763,9 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
         mp[k] = -INFINITY;
         lp[k] = 0.f;
         if (lane + 64 * k < parts) {
-          mp[k] = seq_take(at(r, lane + 64 * k) + cols);
-          lp[k] = seq_take(at(r, lane + 64 * k) + cols + 1);
+          const f32x4 ml = seq_take(ws, at(r, lane + 64 * k) + cols);
+          mp[k] = ml[0];
+          lp[k] = ml[1];
         }
       }
 #pragma unroll
@@ -778,11 +785,11 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
     const bool mine = r < n_rows && 4 * x < cols;
     f32x4 o = f4_zero();
     if (mine) {
-      constexpr int DEEP = 4;  // parts requested together
+      constexpr int DEEP = 8;  // parts requested together
       for (int p = z; p < parts; p += DEEP * side) {
         f32x4 v[DEEP];
 #pragma unroll
-        for (int k = 0; k < DEEP; ++k) v[k] = p + k * side < parts ? seq_take4(at(r, p + k * side) + 4 * x) : f4_zero();
+        for (int k = 0; k < DEEP; ++k) v[k] = p + k * side < parts ? seq_take(ws, at(r, p + k * side) + 4 * x) : f4_zero();
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
           const float f = p + k * side < parts ? weight[y * parts + p + k * side] : 0.f;
@@ -1014,31 +1021,34 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
     const bool bad = PAGED && flag[1] != 0;
     const int cols = a.vchunks * C::E;
     const bool whole = !PAGED || (ta == 0 && tb == u.steps);
-    float* ws = PAGED ? ra.ws + (size_t)(2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4) : nullptr;
+    const unsigned ws = (unsigned)((2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4));
+    const __amdgpu_buffer_rsrc_t to = seq_parts_at(ra.ws);
     bool odd = false;
-    for (int e = threadIdx.x; e < n_rows * cols; e += 256) {
-      const int r = e / cols, d = e - r * cols;
-      float mr = -INFINITY, lr = 0.f, o = 0.f;
+    for (int e = threadIdx.x; e < n_rows * (cols / 4); e += 256) {
+      const int r = e / (cols / 4), d = 4 * (e - r * (cols / 4));
+      float mr = -INFINITY, lr = 0.f;
+      f32x4 o = f4_zero();
 #pragma unroll
       for (int w = 0; w < 4; ++w) mr = fmaxf(mr, ms[32 * w + r]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float mw = ms[32 * w + r];
         lr += mw == -INFINITY ? ls[32 * w + r] : ls[32 * w + r] * __builtin_amdgcn_exp2f((mw - mr) * a.c);
-        o += part[(32 * w + r) * S::PITCH + d];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += part[(32 * w + r) * S::PITCH + d + i];
       }
       if (bad) lr = NAN;
       if (whole) {
-        const float v = lr == 0.f ? 0.f : o / lr;
-        odd |= !(fabsf(v) < INFINITY);
-        const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
-        ((T*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head))[d] = (T)v;
-      } else {
-        seq_give(ws + r * (cols + 4) + d, o);
-        if (d == 0) {
-          seq_give(ws + r * (cols + 4) + cols, mr);
-          seq_give(ws + r * (cols + 4) + cols + 1, lr);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = lr == 0.f ? 0.f : o[i] / lr;
+          odd |= !(fabsf(o[i]) < INFINITY);
         }
+        const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+        *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + d * (int)sizeof(T)) = to_quad<T>(o);
+      } else {
+        seq_give(to, ws + r * (cols + 4) + d, o);
+        if (d == 0) seq_give(to, ws + r * (cols + 4) + cols, f32x4{mr, lr, 0.f, 0.f});
       }
     }
     if (PAGED && !whole) {
@@ -1216,16 +1226,18 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   __syncthreads();
   float l = flag[1] ? -1.f : xor32_sum(st.l);  // -1: of a page that is none
   if (parts > 1) {
-    const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 2) * 64, first = part - p;  // pitch of a wave
-    auto at = [&](int i) __attribute__((always_inline)) { return ra.ws_tiles + (size_t)(first + i) * 4 * pitch + wave * pitch + lane; };
-    float* to = at(p);
+    const int blocks = (a.vchunks * C::E + 31) / 32, pitch = (16 * blocks + 4) * 64, first = part - p;  // pitch of a wave
+    const __amdgpu_buffer_rsrc_t ws = seq_parts_at(ra.ws_tiles);
+    auto at = [&](int i) __attribute__((always_inline)) { return (unsigned)(((first + i) * 4 + wave) * pitch + 4 * lane); };
+    const unsigned to = at(p);
 #pragma unroll
     for (int n = 0; n < C::NMB; ++n)
       if (n < blocks)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) seq_give(to + (16 * n + i) * 64, st.o[n][i]);
-    seq_give(to + (16 * blocks) * 64, st.m);
-    seq_give(to + (16 * blocks + 1) * 64, l);
+        for (int i = 0; i < 4; ++i) {
+          seq_give(ws, to + (4 * n + i) * 256, f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]});
+        }
+    seq_give(ws, to + 4 * blocks * 256, f32x4{st.m, l, 0.f, 0.f});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every storing wave's stores are where the others look
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -1235,21 +1247,25 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
     __syncthreads();
     if (!seq_same(flag[0])) return;
     float m = -INFINITY;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, seq_take(at(i) + (16 * blocks) * 64));
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, seq_take(ws, at(i) + 4 * blocks * 256)[0]);
     st.clear();
     bool none = false;
     l = 0.f;
     for (int i = 0; i < parts; ++i) {
-      const float* from = at(i);
-      const float mp = seq_take(from + (16 * blocks) * 64), lp = seq_take(from + (16 * blocks + 1) * 64);
-      const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mp - m) * a.c);
-      none |= lp < 0.f;
-      l += lp * f;
+      const unsigned from = at(i);
+      const f32x4 ml = seq_take(ws, from + 4 * blocks * 256);
+      const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[0] - m) * a.c);
+      none |= ml[1] < 0.f;
+      l += ml[1] * f;
 #pragma unroll
       for (int n = 0; n < C::NMB; ++n)
-        if (n < blocks)
+        if (n < blocks) {
+          f32x4 v[4];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) st.o[n][j] = __builtin_fmaf(seq_take(from + (16 * n + j) * 64), f, st.o[n][j]);
+          for (int j = 0; j < 4; ++j) v[j] = seq_take(ws, from + (4 * n + j) * 256);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) st.o[n][j] = __builtin_fmaf(v[j / 4][j % 4], f, st.o[n][j]);
+        }
     }
     if (none) l = -1.f;
   }

@@ -133,7 +133,7 @@ extern "C" int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_he
   // counters, two parts of 32 rows a share, and one of 128 rows as four waves hold them where a call can have as many
   const bool tiles = (int64_t)n_tokens * (head_num / kv_head_num) > 32;
   return 4 * (2 * khm::SEQ_SHARES + 2 * khm::SEQ_SHARES * 32 * ((int64_t)value_size + 4) +
-              (tiles ? khm::SEQ_SHARES * (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 2) : 0));
+              (tiles ? khm::SEQ_SHARES * (int64_t)4 * 64 * (16 * ((value_size + 31) / 32) + 4) : 0));
 }
 
 extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, const int32_t* pages, int64_t table_stride,
