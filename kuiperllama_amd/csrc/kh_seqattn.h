@@ -195,10 +195,18 @@ struct SeqState {
     const int r = lane & 31;
     const unsigned at = K + (unsigned)(r * C::RB + 16 * ((lane >> 5) ^ C::turn_k(r)));
     if constexpr (PER == 1) {
+      constexpr int G = C::TIGHT ? 4 : C::NKB;  // requested together, the next ones ahead of these products
+      frag k[2][G];
 #pragma unroll
-      for (int b = 0; b < C::NKB; ++b) {
-        s = Tile32<T>::mma(lds_read<frag>((at ^ (32 * b)) + r0 * C::RB), q[b], s);
-        if (C::TIGHT && b % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < G; ++j) k[0][j] = lds_read<frag>((at ^ (32 * j)) + r0 * C::RB);
+#pragma unroll
+      for (int g = 0; g < C::NKB / G; ++g) {
+        if (g + 1 < C::NKB / G)
+#pragma unroll
+          for (int j = 0; j < G; ++j) k[(g + 1) & 1][j] = lds_read<frag>((at ^ (32 * (G * (g + 1) + j))) + r0 * C::RB);
+#pragma unroll
+        for (int j = 0; j < G; ++j) s = Tile32<T>::mma(k[g & 1][j], q[G * g + j], s);
+        if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       f32x16 small = s;  // apart: as many roundings of the sum as it has blocks
@@ -249,17 +257,25 @@ struct SeqState {
         bf16x8 b;
 #pragma unroll
         for (int i = 0; i < 8; ++i) b[i] = (bf16)p[8 * t + i];
+        constexpr int G = C::TIGHT ? 2 : C::NMB;
+        bf16x8 a[2][G];
+        auto load = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < C::NMB; ++n) {
-          bf16x8 a;
+          for (int j = 0; j < G; ++j)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const bf16x4 v = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)((at ^ (64 * n)) + (r0 + 16 * t + 8 * g) * C::RB)));
+            for (int e = 0; e < 2; ++e) {
+              const bf16x4 v = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)((at ^ (64 * (G * g + j))) + (r0 + 16 * t + 8 * e) * C::RB)));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[4 * g + i] = v[i];
-          }
-          o[n] = Tile32<T>::mma(a, b, o[n]);
-          if (C::TIGHT && n % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+              for (int i = 0; i < 4; ++i) a[g & 1][j][4 * e + i] = v[i];
+            }
+        };
+        load(0);
+#pragma unroll
+        for (int g = 0; g < C::NMB / G; ++g) {
+          if (g + 1 < C::NMB / G) load(g + 1);
+#pragma unroll
+          for (int j = 0; j < G; ++j) o[G * g + j] = Tile32<T>::mma(a[g & 1][j], b, o[G * g + j]);
+          if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
       }
     } else {
