@@ -162,7 +162,8 @@ int kh_scale_sum_f32(const float* value, const float* scale, float* out, int32_t
  * begin.  Rows are described by strides, in elements: [token][head][element], the elements of a head side by side.  A query
  * head h goes with key head h / (head_num / kv_head_num).
  *
- * Types: KH_DTYPE_BF16, KH_DTYPE_F32 (sums, softmax and angles in fp32 or more either way).  Pointers are aligned to 16
+ * Types: KH_DTYPE_BF16, KH_DTYPE_F32 (sums, softmax and angles in fp32 or more either way; attention in fp32 keeps fewer bits
+ * of numbers below 2^-110).  Pointers are aligned to 16
  * bytes; head sizes and strides are multiples of 16 bytes; head_size and value_size are at most 256, a rotation has
  * fewer than 2^24 tokens, attention fewer than 2^30 query rows (tokens times heads).  Anything else is refused:
  * KH_ERR_INVALID_ARG, KH_ERR_UNSUPPORTED for the sizes.  No tokens or no sequences: nothing is done.

@@ -41,7 +41,8 @@ struct Tile32<float> {
 
 // fp32 on the bf16 matrix cores: a number is the sum of three of 8 bits, exactly - rounded to bf16, what is left rounded, what is left then.
 // Of the nine products of two numbers the three smallest are left out, at most 2^-24 of the product each and of either sign: less than the
-// fp32 matrix instruction's own rounding of n sums, for 6 x 32 cycles a block of 16 and not 8 x 64.
+// fp32 matrix instruction's own rounding of n sums, for 6 x 32 cycles a block of 16 and not 8 x 64.  Numbers below 2^-110 have parts below the
+// least there is, and keep fewer bits; those that bf16 has no room for end as no number, and their rows are done again.
 struct Split {
   bf16x8 h, m, l;
 };

@@ -566,6 +566,42 @@ def test_one_workspace_for_calls_of_any_shape(gpu, dtype):
     assert not ws[:4096].any()  # the counters, as the next call needs them
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("max_new", [None, 1], ids=["tiles", "rows"])
+def test_more_new_tokens_than_keys_and_rows_ahead_of_the_first_sequence(gpu, dtype, max_new):
+    """Queries ahead of a sequence's first key get zeros, in tiles and in parts of them; rows that belong to no sequence stay."""
+    from kuiperllama_amd import ops
+    gen = generator(66)
+    H, KH, D, page, ahead = 4, 2, 64, 16, 7
+    new, lens = [200, 150, 90, 1], [70, 0, 2000, 1]
+    kc, vc, table, ks, vs = paged(gen, dtype, KH, D, D, lens, page)
+    q = rnd(gen, dtype, ahead + sum(new) + 4, H, D)
+    out = torch.full_like(q, 9.0)
+    ops.attn_paged(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=gpu), offsets_of(new, gpu) + ahead, out,
+                   ops.attn_paged_workspace(H, KH, D, q.shape[0], gpu), max_new=max_new)
+    check_paged(q[ahead:], out[ahead:], lens, new, ks, vs, 0)
+    assert (out[:ahead] == 9.0).all() and (out[ahead + sum(new):] == 9.0).all()
+    k, v = rnd(gen, dtype, q.shape[0], KH, D), rnd(gen, dtype, q.shape[0], KH, D)
+    out.fill_(9.0)
+    ops.attn_packed(q, k, v, offsets_of(new, gpu) + ahead, out)
+    for b, n in enumerate(new):
+        s = slice(ahead + sum(new[:b]), ahead + sum(new[:b + 1]))
+        close(out[s], *attended(q[s], k[s], v[s], 0, D ** -0.5), f"packed {n}")
+    assert (out[:ahead] == 9.0).all() and (out[ahead + sum(new):] == 9.0).all()
+
+
+@pytest.mark.parametrize("power", [-100, 100])
+def test_fp32_of_any_size(gpu, power):
+    """Values near both ends of the exponents: as exact as those near one."""
+    from kuiperllama_amd import ops
+    gen = generator(14)
+    n, H, D = 130, 2, 64
+    q, k, v = rnd(gen, F32, n, H, D), rnd(gen, F32, n, H, D), rnd(gen, F32, n, H, D)
+    want, bound = attended(q, k, v, 0, D ** -0.5)
+    out = ops.attn_packed(q * 2.0 ** -60, k * 2.0 ** 60, v * 2.0 ** power, offsets_of([n], gpu), torch.empty_like(q))
+    close(out.double() * 2.0 ** -power, want, bound)
+
+
 def test_another_stream_and_the_same_answer_twice(gpu):
     from kuiperllama_amd import ops
     gen = generator(12)
