@@ -14,7 +14,7 @@
 // a score passes it by 8 / c: weights then stay below 2^8, which fp32 sums and products in bf16 hold as well as those below one,
 // and most tiles spare the output its factor.
 // Roundings: scores, weights, sums and outputs are fp32; for bf16 the weights are rounded to bf16 for their product with the
-// values (the sum l takes them unrounded).
+// values (the sum l takes them unrounded).  fp32 operands are split, not rounded (Split).
 #pragma once
 #include "kh_lgemm.h"
 
@@ -117,11 +117,11 @@ template <class T, int DP>
 struct SeqCfg {
   static constexpr int E = 16 / (int)sizeof(T);
   static constexpr int RB = (DP <= 64 ? 64 : (DP <= 128 ? 128 : 256)) * (int)sizeof(T);  // bytes of a staged row
-  static constexpr int CB = RB / 16;              // its chunks
+  static constexpr int CB = RB / 16;                    // its chunks
   static constexpr int NKB = DP * (int)sizeof(T) / 32;  // 32-byte k-blocks
-  static constexpr int NMB = DP / 32;             // 32-column blocks of the output
+  static constexpr int NMB = DP / 32;                   // 32-column blocks of the output
   static constexpr bool TIGHT = RB > 256 || sizeof(T) == 4;  // queries and outputs fill the registers: reads of LDS stay near their use
-  static constexpr bool HOLD = RB <= 512;         // queries in registers; else read again for each tile, under 128 products of 64 cycles
+  static constexpr bool HOLD = RB <= 512;                    // queries in registers; else read, and split, again for each tile
   // LDS: chunk c of row r of the keys lies in slot c ^ turn_k(r), of the values in c ^ turn_v(r).  Reads of 16 bytes of 16 rows
   // (keys), of 32 bytes of four rows (values) then touch every bank once.  turn_v(r + 8) = turn_v(r), turn_v(4 + i) = turn_v(4) ^ turn_v(i),
   // turn_k(r + 16) = turn_k(r): a lane's addresses of a tile are one of its own, turned by constants.
@@ -453,7 +453,7 @@ struct SeqTiles {
   static constexpr int RING = 4 * TB;                // two tiles of keys and values each
   static constexpr int MOST = 1024;                  // slots that are looked at to be cut
   static constexpr int LDS_PACKED = RING, LDS_PAGED = RING + 4 * SEQ_TAB + 64, LDS_SHARES = LDS_PAGED + 4 * (MOST + 4);
-  static constexpr int LEAST = 512 / BN;             // steps of a part
+  static constexpr int LEAST = 512 / BN;             // steps of a part: 64 tokens behind 4032 keys 33 us, by 256 keys 38, by 1024 37
 };
 
 // 128 query rows of a key head, as one of four waves sees them.
