@@ -14,7 +14,8 @@
 // a score passes it by 8 / c: weights then stay below 2^8, which fp32 sums and products in bf16 hold as well as those below one,
 // and most tiles spare the output its factor.
 // Roundings: scores, weights, sums and outputs are fp32; for bf16 the weights are rounded to bf16 for their product with the
-// values (the sum l takes them unrounded).  fp32 operands are split, not rounded (Split).
+// values, and l is the sum of the rounded ones: what is divided by it is a mean of the values, in which a weight's rounding weighs
+// (v_j - out) and not v_j, so that a key that outweighs the others comes out as it is.  fp32 operands are split, not rounded (Split).
 #pragma once
 #include "kh_lgemm.h"
 
@@ -23,6 +24,7 @@
 namespace khm {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // 32 x 32 products of 32-byte k-blocks.  A fragment is 16 bytes a lane: row l & 31, bytes [16 (l / 32), + 16) of the block.
 template <class T>
@@ -160,6 +162,31 @@ struct SeqState {
   int chunks;
   f32x16 o[C::NMB];
   float m, l;  // l: this half's keys
+  struct Rounded {  // the weights of 32 keys as their product with the values takes them
+    bf16x8 p[2];
+  };
+  typedef typename std::conditional<sizeof(T) == 2, Rounded, f32x16>::type weights;
+  // in the registers of the scores that they were
+  static __device__ __forceinline__ f32x16 held(const weights& w) {
+    if constexpr (sizeof(T) == 2) {
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = __builtin_bit_cast(f32x4, w.p[i / 4])[i % 4];
+      return s;
+    } else {
+      return w;
+    }
+  }
+  static __device__ __forceinline__ weights taken(const f32x16& s) {
+    if constexpr (sizeof(T) == 2) {
+      weights w;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) w.p[i] = __builtin_bit_cast(bf16x8, f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]});
+      return w;
+    } else {
+      return s;
+    }
+  }
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -236,28 +263,37 @@ struct SeqState {
         for (int i = 0; i < 16; ++i) o[n][i] *= f;
     }
   }
-  __device__ __forceinline__ f32x16 weigh(const f32x16& s, float c) {
+  __device__ __forceinline__ weights weigh(const f32x16& s, float c) {
     const float base = m == -INFINITY ? 0.f : -m * c;  // no key seen yet: 2^-inf
     f32x16 p;
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, base));
     float t = 0.f;
+    if constexpr (sizeof(T) == 2) {
+      weights w;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += p[i];
-    l += t;
-    return p;
+      for (int i = 0; i < 16; ++i) w.p[i / 8][i % 8] = (bf16)p[i];
+      // two of them a sum, off by 2^-23 of it at most
+      const bf16x2 ones = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) t = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w.p[i / 8][i % 8], w.p[i / 8][i % 8 + 1]}, ones, t, false);
+      l += t;
+      return w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t += p[i];
+      l += t;
+      return p;
+    }
   }
   // O^T += V^T P^T for 32 keys, rows r0 .. of the tile at V
-  __device__ __forceinline__ void add(const f32x16& p, unsigned V, int r0, int lane) {
+  __device__ __forceinline__ void add(const weights& w, unsigned V, int r0, int lane) {
     const int half = lane >> 5;
     if constexpr (sizeof(T) == 2) {
       const int r = 4 * half + ((lane >> 2) & 3);  // of eight
       const unsigned at = V + (unsigned)(r * C::RB + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ C::turn_v(r)) + 8 * (lane & 1));
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        bf16x8 b;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = (bf16)p[8 * t + i];
         constexpr int G = C::TIGHT ? 2 : C::NMB;
         bf16x8 a[2][G];
         auto load = [&](int g) __attribute__((always_inline)) {
@@ -275,7 +311,7 @@ struct SeqState {
         for (int g = 0; g < C::NMB / G; ++g) {
           if (g + 1 < C::NMB / G) load(g + 1);
 #pragma unroll
-          for (int j = 0; j < G; ++j) o[G * g + j] = Tile32<T>::mma(a[g & 1][j], b, o[G * g + j]);
+          for (int j = 0; j < G; ++j) o[G * g + j] = Tile32<T>::mma(a[g & 1][j], w.p[t], o[G * g + j]);
           if (C::TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -283,10 +319,10 @@ struct SeqState {
       const unsigned at = V + (unsigned)(4 * half * C::RB + 16 * (((lane & 31) >> 2) ^ C::turn_v(4 * half)) + 4 * (lane & 3));
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        float w[8];
+        float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = p[8 * t + j];
-        const Split x = seq_split(w);
+        for (int j = 0; j < 8; ++j) p[j] = w[8 * t + j];
+        const Split x = seq_split(p);
 #pragma unroll
         for (int n = 0; n < C::NMB; ++n) {
           float v[8];
@@ -1005,10 +1041,10 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
           st.follow(xor32_max(mx), a.c);
-          s = st.weigh(s, a.c);
+          s = SeqState<T, DP>::held(st.weigh(s, a.c));
         }
         landed(h + 1);
-        if (some) st.add(s, ring + (unsigned)((h + 1) % S::NB * S::TB), 0, lane);
+        if (some) st.add(SeqState<T, DP>::taken(s), ring + (unsigned)((h + 1) % S::NB * S::TB), 0, lane);
         used(h + 1);
       }
     }

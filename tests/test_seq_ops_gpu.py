@@ -673,3 +673,41 @@ def test_refusals_on_the_device(gpu):
                        (dict(k=f(4, 3, 64), v=f(4, 3, 64)), _ffi.KhError), (dict(q=f(4, 4, 320), k=f(4, 2, 320)), _ffi.KhError)):
         with pytest.raises(error):
             ops.attn_packed(**{**ok, **bad})
+
+
+# ---- every way that a call can be dealt ------------------------------------------------------------------------------------
+def every_form(q, k, v, **kw):
+    """One sequence, as a whole prompt (150 tokens: tiles, 900: blocks of 32 rows), as the last two thirds of it over pages in tiles and in
+    rows, its last token alone.  -> name, first token, out"""
+    from kuiperllama_amd import ops
+    n, H = q.shape[:2]
+    KH, DV = v.shape[1:]
+    yield "packed", 0, ops.attn_packed(q, k, v, offsets_of([n], q.device), torch.full((n, H, DV), 9.0, dtype=q.dtype, device=q.device), **kw)
+    page, j = 16, torch.arange(n, device=q.device)
+    held = -(-n // page)
+    at = held - 1 - j // page, j % page  # the pages from behind
+    kc, vc = (torch.full((held, page, KH, x.shape[2]), math.nan, dtype=q.dtype, device=q.device) for x in (k, v))
+    kc[at], vc[at] = k, v
+    table = torch.arange(held - 1, -1, -1, dtype=torch.int32, device=q.device)[None]
+    length = torch.tensor([n], dtype=torch.int32, device=q.device)
+    for name, new, most in (("portion", n - n // 3, None), ("rows", n - n // 3, 1), ("last", 1, 1)):
+        out = torch.full((new, H, DV), 9.0, dtype=q.dtype, device=q.device)
+        ws = ops.attn_paged_workspace(H, KH, DV, new, q.device)
+        yield name, n - new, ops.attn_paged(q[n - new:], kc, vc, table, length, offsets_of([new], q.device), out, ws, max_new=most, **kw)
+
+
+@pytest.mark.parametrize("n", [150, 900], ids=["tiles", "blocks"])
+def test_weights_add_up_to_one(gpu, n):
+    """Values that are the same in every token come out as they are, whatever bf16 makes of the weights: their sum is taken of the rounded ones.
+    One key outweighs the others by 2^2 to 2^3 and comes after a tile of theirs, so that its own weight is no power of two and is rounded.
+    The sums of n terms are off by 2 n u of the value at most (900: 1.1e-4), and a value's nearest other rounding is 2^-9 of it away."""
+    gen = generator(91)
+    H, KH, D = 16, 16, 64
+    q, k = torch.zeros(n, H, D, dtype=BF16, device=gpu), torch.zeros(n, KH, D, dtype=BF16, device=gpu)
+    q[..., 0] = 1
+    k[..., 0] = -20
+    k[0, :, 0] = 0
+    k[130, :, 0] = 2 + (2 * torch.arange(KH, device=gpu) + 1) / 64
+    v = rnd(gen, BF16, 1, KH, D).expand(n, -1, -1).contiguous()
+    for name, first, out in every_form(q, k, v, scale=math.log(2.0)):
+        assert torch.equal(out, v[first:]), name
