@@ -44,7 +44,8 @@ SeqArgs args_of(const kh_attn_rows* r, int e) {
   a.group = r->head_num / r->kv_head_num;
   a.kchunks = r->head_size * e / 16;
   a.vchunks = r->value_size * e / 16;
-  a.window = r->window;
+  // places and lengths stay below 2^30 either way: a window of more holds everything, and a place less one of no more has room in 32 bits
+  a.window = r->window > INT_MAX / 2 ? 0 : r->window;
   a.c = r->scale * 1.4426950408889634f;
   return a;
 }

@@ -711,3 +711,23 @@ def test_weights_add_up_to_one(gpu, n):
     v = rnd(gen, BF16, 1, KH, D).expand(n, -1, -1).contiguous()
     for name, first, out in every_form(q, k, v, scale=math.log(2.0)):
         assert torch.equal(out, v[first:]), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("max_new", [None, 1], ids=["tiles", "rows"])
+def test_a_window_that_holds_everything(gpu, dtype, max_new):
+    """The largest int32 as a window, with queries ahead of their sequence's first key too: as no window."""
+    from kuiperllama_amd import ops
+    gen = generator(67)
+    H, KH, D, page = 4, 2, 64, 16
+    new, lens = [200, 150, 90, 1], [70, 0, 2000, 30]
+    kc, vc, table, ks, vs = paged(gen, dtype, KH, D, D, lens, page)
+    q = rnd(gen, dtype, sum(new), H, D)
+    ws = ops.attn_paged_workspace(H, KH, D, q.shape[0], gpu)
+    args = (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=gpu), offsets_of(new, gpu))
+    want = ops.attn_paged(*args, torch.full_like(q, 9.0), ws, max_new=max_new)
+    check_paged(q, want, lens, new, ks, vs, 0)
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 2 ** 30 - 1, 5000):
+        out = ops.attn_paged(*args, torch.full_like(q, 9.0), ws, max_new=max_new, window=window)
+        check_paged(q, out, lens, new, ks, vs, 0, f"window {window}")
+        assert torch.equal(out, want), window
