@@ -425,7 +425,8 @@ __device__ __forceinline__ int seq_table(const SeqKv& kv, const int32_t* table, 
 
 // One query by one wave from global memory, 64 keys at a time: a lane has a key for the scores, four columns for the output.  A key
 // that the query does not see is not touched, so that what it holds cannot reach it (in a product over a tile it is zero times
-// the value, which is no zero for what is no number): for the rows where that seems to have happened.
+// the value, which is no zero for what is no number): for the rows where that seems to have happened, and for those whose weights
+// add up to nothing though they see a key - its place is theirs - for want of a score above minus infinity: NaN, as of the formula.
 template <class T, bool PAGED>
 __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char* q, char* out, int place, int lane) {
   typedef typename Tile<T>::frag frag;
@@ -457,7 +458,7 @@ __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char
         if (lane + 64 * i < cols && w != 0.f) o[i] = __builtin_fmaf(w, (float)((const T*)row)[lane + 64 * i], o[i]);
     }
   }
-  const float f = __builtin_amdgcn_ballot_w64(x.bad) ? NAN : (l == 0.f ? 0.f : 1.0f / l);
+  const float f = __builtin_amdgcn_ballot_w64(x.bad) || (l == 0.f && place >= 0) ? NAN : (l == 0.f ? 0.f : 1.0f / l);
   for (int i = 0; i < 4; ++i)
     if (lane + 64 * i < cols) ((T*)out)[lane + 64 * i] = (T)(o[i] * f);
 }
@@ -636,7 +637,7 @@ __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, con
         if (d < a.vchunks * C::E) *(typename Tile<T>::quad*)(out + d * (int)sizeof(T)) = to_quad<T>(v);
       }
   }
-  if (__builtin_amdgcn_ballot_w64(!bad && st.odd())) {
+  if (__builtin_amdgcn_ballot_w64(!bad && (st.odd() || (l == 0.f && s.place >= 0)))) {
     wait_vm<0>();  // what is above is written
     s.x.bad = false;
     for (int r = s.w0; r < s.w0 + 32 && r < s.rows; ++r) {
@@ -860,12 +861,13 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
         for (int i = 0; i < 4; ++i) o[i] += v[i];
       }
       const float l = ls[r];
+      const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+      odd |= l == 0.f && u.sp.length - u.sp.n + tk >= 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[i] = l == 0.f ? 0.f : o[i] / l;
         odd |= !(fabsf(o[i]) < INFINITY);
       }
-      const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
       *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + 4 * x * (int)sizeof(T)) = to_quad<T>(o);
     }
     __syncthreads();
@@ -1092,12 +1094,13 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
       }
       if (bad) lr = NAN;
       if (whole) {
+        const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
+        odd |= lr == 0.f && u.sp.length - u.sp.n + tk >= 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           o[i] = lr == 0.f ? 0.f : o[i] / lr;
           odd |= !(fabsf(o[i]) < INFINITY);
         }
-        const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
         *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + d * (int)sizeof(T)) = to_quad<T>(o);
       } else {
         seq_give(to, ws + r * (cols + 4) + d, o);

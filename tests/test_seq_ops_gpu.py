@@ -731,3 +731,31 @@ def test_a_window_that_holds_everything(gpu, dtype, max_new):
         out = ops.attn_paged(*args, torch.full_like(q, 9.0), ws, max_new=max_new, window=window)
         check_paged(q, out, lens, new, ks, vs, 0, f"window {window}")
         assert torch.equal(out, want), window
+
+
+BOTH = [pytest.mark.parametrize("n", [150, 900], ids=["tiles", "blocks"]), pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])]
+
+
+def both(f):
+    for mark in BOTH:
+        f = mark(f)
+    return f
+
+
+@both
+def test_scores_that_are_all_minus_infinity(gpu, dtype, n):
+    """A query that sees keys, every one of them at minus infinity, has no softmax: NaN, as the formula says, and not the zeros of a query that
+    sees none.  One finite key is enough."""
+    gen = generator(92)
+    H, KH, D, t = 4, 2, 64, 100
+    q, k, v = rnd(gen, dtype, n, H, D), rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, D)
+    q[..., 0] = q[..., 0].abs() + 1
+    k[:t, :, 0] = -math.inf
+    want, bound = attended(q[t:], k[t:], v[t:], 0, D ** -0.5)
+    for name, first, out in every_form(q, k, v):
+        none = max(0, t - first)
+        assert torch.isnan(out[:none]).all(), name
+        close(out[none:], want[first + none - t:], bound[first + none - t:], name)
+    k[:, :, 0] = -math.inf
+    for name, first, out in every_form(q, k, v):
+        assert torch.isnan(out).all(), name
