@@ -455,7 +455,7 @@ __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char
       const float w = __shfl(p, j);
       const char* row = x.v + __shfl((long long)vo, j);
       for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < cols && w != 0.f) o[i] = __builtin_fmaf(w, (float)((const T*)row)[lane + 64 * i], o[i]);
+        if (lane + 64 * i < cols) o[i] = __builtin_fmaf(w, (float)((const T*)row)[lane + 64 * i], o[i]);
     }
   }
   const float f = __builtin_amdgcn_ballot_w64(x.bad) || (l == 0.f && place >= 0) ? NAN : (l == 0.f ? 0.f : 1.0f / l);

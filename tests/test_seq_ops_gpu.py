@@ -759,3 +759,20 @@ def test_scores_that_are_all_minus_infinity(gpu, dtype, n):
     k[:, :, 0] = -math.inf
     for name, first, out in every_form(q, k, v):
         assert torch.isnan(out).all(), name
+
+
+@both
+def test_an_infinity_of_a_weight_that_vanishes(gpu, dtype, n):
+    """A key that a query sees, of a weight that fp32 has no number for: its infinity is not lost."""
+    gen = generator(94)
+    H, KH, D, t = 4, 2, 64, 5
+    q, k, v = torch.zeros(n, H, D, dtype=dtype, device=gpu), torch.zeros(n, KH, D, dtype=dtype, device=gpu), rnd(gen, dtype, n, KH, D)
+    q[..., 0] = 1
+    k[t, :, 0] = -300
+    want, bound = attended(q, k, v, 0, 1.0)
+    v[t, :, ::3] = math.inf
+    hit = torch.zeros(n, H, D, dtype=torch.bool, device=gpu)
+    hit[t:, :, ::3] = True
+    for name, first, out in every_form(q, k, v, scale=1.0):
+        assert not torch.isfinite(out[hit[first:]]).any(), name
+        close(out[~hit[first:]], want[first:][~hit[first:]], bound[first:][~hit[first:]], name)
