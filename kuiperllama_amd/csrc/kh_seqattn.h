@@ -423,44 +423,68 @@ __device__ __forceinline__ int seq_table(const SeqKv& kv, const int32_t* table, 
   return p0;
 }
 
-// One query by one wave from global memory, 64 keys at a time: a lane has a key for the scores, four columns for the output.  A key
-// that the query does not see is not touched, so that what it holds cannot reach it (in a product over a tile it is zero times
-// the value, which is no zero for what is no number): for the rows where that seems to have happened, and for those whose weights
-// add up to nothing though they see a key - its place is theirs - for want of a score above minus infinity: NaN, as of the formula.
+// One query by one wave from global memory, 64 keys at a time, in two passes: the maximum and the sum of the weights, then the values,
+// each with its weight over that sum, which is at most 1 - so that no sum of them passes what a number holds where their mean does not.
+// A lane has a key for the scores, four columns for the output.  A key that the query does not see is not touched, so that what
+// it holds cannot reach it (in a product over a tile it is zero times the value, which is no zero for what is no number): for the
+// rows where that seems to have happened, and for those whose weights add up to nothing though they see a key - its place is theirs -
+// for want of a score above minus infinity: NaN, as of the formula.
 template <class T, bool PAGED>
 __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char* q, char* out, int place, int lane) {
   typedef typename Tile<T>::frag frag;
-  constexpr int E = Tile<T>::N;
+  constexpr int E = Tile<T>::N, DEEP = 8;  // values requested together
   const int lo = a.window > 0 && place >= a.window ? place - a.window + 1 : 0, cols = a.vchunks * E;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = lo; k0 <= place; k0 += 64) {
-    const int key = k0 + lane;
-    int64_t ko = 0, vo = 0;
+  auto score = [&](int key, int64_t& vo) __attribute__((always_inline)) {
     float s = -INFINITY;
     if (key <= place) {
+      int64_t ko;
       seq_row<PAGED>(a, x, key, ko, vo);
       s = 0.f;
+#pragma unroll 4
       for (int c = 0; c < a.kchunks; ++c) {
         const frag u = *(const frag*)(q + 16 * c), w = *(const frag*)(x.k + ko + 16 * c);
         for (int i = 0; i < E; ++i) s = __builtin_fmaf((float)u[i], (float)w[i], s);
       }
     }
-    const float to = fmaxf(m, wave_max(s)), base = to == -INFINITY ? 0.f : -to * a.c;
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * a.c), p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c, base));
-    m = to;
-    l = l * f + wave_sum(p);
-    for (int i = 0; i < 4; ++i) o[i] *= f;
-    const int n = place - k0 < 63 ? place - k0 + 1 : 64;
-    for (int j = 0; j < n; ++j) {
-      const float w = __shfl(p, j);
-      const char* row = x.v + __shfl((long long)vo, j);
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < cols) o[i] = __builtin_fmaf(w, (float)((const T*)row)[lane + 64 * i], o[i]);
+    return s;
+  };
+  float m = -INFINITY, l = 0.f;  // l: this lane's keys
+  auto weight = [&](float s) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c, m == -INFINITY ? 0.f : -m * a.c)); };
+  int64_t vo = 0;
+  for (int k0 = lo; k0 <= place; k0 += 64) {
+    const float s = score(k0 + lane, vo), before = m;
+    m = fmaxf(m, wave_max(s));
+    l = l * (before == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((before - m) * a.c)) + weight(s);
+  }
+  l = wave_sum(l);
+  const bool bad = __builtin_amdgcn_ballot_w64(x.bad) != 0;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (bad || l != l || (l == 0.f && place >= 0)) {
+    for (int i = 0; i < 4; ++i) o[i] = NAN;
+  } else if (l != 0.f) {
+    const float share = 1.0f / l;
+    for (int k0 = lo; k0 <= place; k0 += 64) {
+      const float p = weight(score(k0 + lane, vo)) * share;
+      const int n = place - k0 < 63 ? place - k0 + 1 : 64;
+      for (int j0 = 0; j0 < n; j0 += DEEP) {
+        float v[DEEP][4];
+#pragma unroll
+        for (int j = 0; j < DEEP; ++j) {
+          const T* row = (const T*)(x.v + __shfl((long long)vo, j0 + j));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = j0 + j < n && lane + 64 * i < cols ? (float)row[lane + 64 * i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < DEEP; ++j) {
+          const float w = __shfl(p, j0 + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, v[j][i], o[i]);
+        }
+      }
     }
   }
-  const float f = __builtin_amdgcn_ballot_w64(x.bad) || (l == 0.f && place >= 0) ? NAN : (l == 0.f ? 0.f : 1.0f / l);
   for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < cols) ((T*)out)[lane + 64 * i] = (T)(o[i] * f);
+    if (lane + 64 * i < cols) ((T*)out)[lane + 64 * i] = (T)o[i];
 }
 
 // The sequence whose slots hold slot i, where sequence b has the slots from offsets[b] G / BM + b on: at least as many as it has

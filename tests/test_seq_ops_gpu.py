@@ -776,3 +776,18 @@ def test_an_infinity_of_a_weight_that_vanishes(gpu, dtype, n):
     for name, first, out in every_form(q, k, v, scale=1.0):
         assert not torch.isfinite(out[hit[first:]]).any(), name
         close(out[~hit[first:]], want[first:][~hit[first:]], bound[first:][~hit[first:]], name)
+
+
+@both
+def test_means_of_values_near_the_largest_number(gpu, dtype, n):
+    """Values of 2^127 to 1.9 2^127: their sum has no room in fp32, their mean has."""
+    gen = generator(93)
+    H, KH, D = 4, 2, 64
+    q, k = rnd(gen, dtype, n, H, D), rnd(gen, dtype, n, KH, D)
+    v = (1 + 0.9 * torch.rand(n, KH, D, device=gpu, generator=gen)) * 2.0 ** 127
+    v[..., 1::2] *= (torch.rand(n, KH, D // 2, device=gpu, generator=gen) < 0.5) * 2.0 - 1
+    v = v.to(dtype)
+    want, bound = attended(q, k, v, 0, D ** -0.5)
+    for name, first, out in every_form(q, k, v):
+        assert torch.isfinite(out).all(), name
+        close(out, want[first:], bound[first:], name)
