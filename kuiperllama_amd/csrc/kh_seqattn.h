@@ -427,8 +427,8 @@ __device__ __forceinline__ int seq_table(const SeqKv& kv, const int32_t* table, 
 // each with its weight over that sum, which is at most 1 - so that no sum of them passes what a number holds where their mean does not.
 // A lane has a key for the scores, four columns for the output.  A key that the query does not see is not touched, so that what
 // it holds cannot reach it (in a product over a tile it is zero times the value, which is no zero for what is no number): for the
-// rows where that seems to have happened, and for those whose weights add up to nothing though they see a key - its place is theirs -
-// for want of a score above minus infinity: NaN, as of the formula.
+// rows where that seems to have happened, and for those whose weights add up to nothing though they see a key (its place is theirs):
+// c times their scores has no room in a number, or all of these are minus infinity, and the row is NaN, as of the formula.
 template <class T, bool PAGED>
 __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char* q, char* out, int place, int lane) {
   typedef typename Tile<T>::frag frag;
@@ -449,7 +449,8 @@ __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char
     return s;
   };
   float m = -INFINITY, l = 0.f;  // l: this lane's keys
-  auto weight = [&](float s) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c, m == -INFINITY ? 0.f : -m * a.c)); };
+  // the scores' difference first: c times a score may have no room
+  auto weight = [&](float s) __attribute__((always_inline)) { return s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s - m) * a.c); };
   int64_t vo = 0;
   for (int k0 = lo; k0 <= place; k0 += 64) {
     const float s = score(k0 + lane, vo), before = m;

@@ -791,3 +791,17 @@ def test_means_of_values_near_the_largest_number(gpu, dtype, n):
     for name, first, out in every_form(q, k, v):
         assert torch.isfinite(out).all(), name
         close(out, want[first:], bound[first:], name)
+
+
+@both
+def test_scores_near_the_largest_number(gpu, dtype, n):
+    """Scores of 3e38 that are all alike have equal weights; smaller ones beside them have none."""
+    gen = generator(95)
+    H, KH, D = 4, 2, 64
+    q, k, v = torch.zeros(n, H, D, dtype=dtype, device=gpu), torch.zeros(n, KH, D, dtype=dtype, device=gpu), rnd(gen, dtype, n, KH, D)
+    q[..., 0] = 2.0 ** 64
+    k[..., 0] = 1.75 * 2.0 ** 63
+    k[1::3, :, 0] = -(2.0 ** 63)
+    want, bound = attended(torch.ones_like(q[..., :1]), (k[..., :1] > 0).to(dtype) * 1000, v, 0, 1.0)
+    for name, first, out in every_form(q, k, v, scale=1.0):
+        close(out, want[first:], bound[first:], name)
