@@ -644,7 +644,7 @@ __device__ __forceinline__ void seq_tile_run(const SeqArgs& a, const SeqTile& s,
     }
   }
 }
-// The wave's 32 rows, l being those of both halves; rows with what is no number once more, with care.
+// The wave's 32 rows, l being those of both halves; rows with what is no number, and they alone, once more, with care.
 template <class T, int DP, bool PAGED>
 __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, const SeqState<T, DP>& st, float l, bool bad, int lane) {
   typedef SeqCfg<T, DP> C;
@@ -662,11 +662,12 @@ __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, con
         if (d < a.vchunks * C::E) *(typename Tile<T>::quad*)(out + d * (int)sizeof(T)) = to_quad<T>(v);
       }
   }
-  if (__builtin_amdgcn_ballot_w64(!bad && (st.odd() || (l == 0.f && s.place >= 0)))) {
+  const uint64_t odd = __builtin_amdgcn_ballot_w64(!bad && s.row < s.rows && (st.odd() || (l == 0.f && s.place >= 0)));
+  if (odd) {
     wait_vm<0>();  // what is above is written
     s.x.bad = false;
-    for (int r = s.w0; r < s.w0 + 32 && r < s.rows; ++r) {
-      const int tk = r / a.group, hd = s.head * a.group + r - tk * a.group;
+    for (uint32_t left = (uint32_t)(odd | odd >> 32); left; left &= left - 1) {
+      const int r = s.w0 + __builtin_ctz(left), tk = r / a.group, hd = s.head * a.group + r - tk * a.group;
       seq_one<T, PAGED>(a, s.x, a.q + (s.sp.first + tk) * a.q_token + hd * a.q_head, a.out + (s.sp.first + tk) * a.o_token + hd * a.o_head,
                         s.sp.length - s.sp.n + tk, lane);
     }
@@ -793,12 +794,12 @@ struct SeqRows {
   static constexpr int SHARES = LDS <= 80 * 1024 ? SEQ_SHARES : SEQ_SHARES / 2;
 };
 
-// The final rows of a unit: o / l, and with care where that is no number.
+// Rows of a unit, a bit each, once more with care, by the waves in turn.
 template <class T, bool PAGED>
-__device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, int b, int head, int r0, int rows, bool odd, int wave, int lane) {
-  if (!odd) return;
-  for (int r = r0 + wave; r < r0 + rows; r += 4) {
-    const int tk = r / a.group, h = head * a.group + r - tk * a.group, place = u.sp.length - u.sp.n + tk;
+__device__ __forceinline__ void seq_finish(const SeqArgs& a, const SeqUnits& u, int b, int head, int r0, uint32_t odd, int wave, int lane) {
+  for (int i = 0; odd; ++i, odd &= odd - 1) {
+    if (i % 4 != wave) continue;
+    const int r = r0 + __builtin_ctz(odd), tk = r / a.group, h = head * a.group + r - tk * a.group, place = u.sp.length - u.sp.n + tk;
     SeqKeys x = seq_keys(a, b, head, u.sp, place, place);
     seq_one<T, PAGED>(a, x, a.q + (u.sp.first + tk) * a.q_token + h * a.q_head, a.out + (u.sp.first + tk) * a.o_token + h * a.o_head, place, lane);
   }
@@ -818,9 +819,9 @@ __device__ __forceinline__ f32x4 seq_take(__amdgpu_buffer_rsrc_t from, unsigned 
 }
 
 // The rows of a unit from its parts: their weights (LDS, as many rows at a time as fit `room` floats), then their outputs, four columns a
-// thread and as many parts side by side as there are threads.  True where an output is no number.
+// thread and as many parts side by side as there are threads.  -> this thread's rows, a bit each, whose output is no number
 template <class T>
-__device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& u, int head, int r0, int n_rows, int i0, int parts, float* weight,
+__device__ __forceinline__ uint32_t seq_join(const SeqRowsArgs& ra, const SeqUnits& u, int head, int r0, int n_rows, int i0, int parts, float* weight,
                                          int room, float* ls, f32x4* red, int wave, int lane) {
   const SeqArgs& a = ra.s;
   const int cols = a.vchunks * (16 / (int)sizeof(T)), pitch = cols + 4;
@@ -832,7 +833,7 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
   while (down < n_rows && down * across < 256 && 2 * down * parts <= room) down *= 2;
   const int side = 256 / (across * down), x = (int)threadIdx.x & (across - 1), y = (int)threadIdx.x / across & (down - 1),
             z = (int)threadIdx.x / (across * down);
-  bool odd = false;
+  uint32_t odd = 0;
   for (int rb = 0; rb < n_rows; rb += down) {
     for (int r = rb + wave; r < rb + down && r < n_rows; r += 4) {
       constexpr int PER = SEQ_SHARES / 64;
@@ -887,12 +888,13 @@ __device__ __forceinline__ bool seq_join(const SeqRowsArgs& ra, const SeqUnits& 
       }
       const float l = ls[r];
       const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
-      odd |= l == 0.f && u.sp.length - u.sp.n + tk >= 0;
+      bool again = l == 0.f && u.sp.length - u.sp.n + tk >= 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[i] = l == 0.f ? 0.f : o[i] / l;
-        odd |= !(fabsf(o[i]) < INFINITY);
+        again |= !(fabsf(o[i]) < INFINITY);
       }
+      odd |= (uint32_t)again << r;
       *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + 4 * x * (int)sizeof(T)) = to_quad<T>(o);
     }
     __syncthreads();
@@ -1081,7 +1083,8 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
       ms[32 * wave + lane] = st.m;
       ls[32 * wave + lane] = l;
     }
-    __syncthreads();  // everyone is done with the ring
+    __syncthreads();  // everyone is done with the ring, and with the rows of the unit before
+    if (threadIdx.x == 0) flag[4] = 0;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[32 * w + (lane & 31)]);
@@ -1103,7 +1106,7 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
     const bool whole = !PAGED || (ta == 0 && tb == u.steps);
     const unsigned ws = (unsigned)((2 * share + (ta == 0 ? 1 : 0)) * 32 * (cols + 4));
     const __amdgpu_buffer_rsrc_t to = seq_parts_at(ra.ws);
-    bool odd = false;
+    uint32_t odd = 0;
     for (int e = threadIdx.x; e < n_rows * (cols / 4); e += 256) {
       const int r = e / (cols / 4), d = 4 * (e - r * (cols / 4));
       float mr = -INFINITY, lr = 0.f;
@@ -1120,12 +1123,13 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
       if (bad) lr = NAN;
       if (whole) {
         const int tk = (r0 + r) / a.group, hd = head * a.group + r0 + r - tk * a.group;
-        odd |= lr == 0.f && u.sp.length - u.sp.n + tk >= 0;
+        bool again = lr == 0.f && u.sp.length - u.sp.n + tk >= 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           o[i] = lr == 0.f ? 0.f : o[i] / lr;
-          odd |= !(fabsf(o[i]) < INFINITY);
+          again |= !(fabsf(o[i]) < INFINITY);
         }
+        odd |= (uint32_t)again << r;
         *(typename Tile<T>::quad*)(a.out + (u.sp.first + tk) * a.o_token + hd * a.o_head + d * (int)sizeof(T)) = to_quad<T>(o);
       } else {
         seq_give(to, ws + r * (cols + 4) + d, o);
@@ -1146,11 +1150,9 @@ __device__ __forceinline__ void seq_rows(const SeqRowsArgs& ra, int shares, int 
       odd = seq_join<T>(ra, u, head, r0, n_rows, i0, parts, (float*)smem_raw, S::RING / 4, ls, (f32x4*)tab, wave, lane);
       tab_b = -1;
     }
-    const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (lane == 0) flag[4 + wave] = any;
+    if (odd) __hip_atomic_fetch_or((uint32_t*)flag + 4, odd, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     __syncthreads();
-    odd = flag[4] | flag[5] | flag[6] | flag[7];
-    seq_finish<T, PAGED>(a, u, b, head, r0, n_rows, odd, wave, lane);
+    seq_finish<T, PAGED>(a, u, b, head, r0, (uint32_t)seq_same(flag[4]), wave, lane);
   }
 }
 

@@ -805,3 +805,16 @@ def test_scores_near_the_largest_number(gpu, dtype, n):
     want, bound = attended(torch.ones_like(q[..., :1]), (k[..., :1] > 0).to(dtype) * 1000, v, 0, 1.0)
     for name, first, out in every_form(q, k, v, scale=1.0):
         close(out, want[first:], bound[first:], name)
+
+
+@both
+def test_a_query_that_is_no_number_leaves_the_others_as_they_are(gpu, dtype, n):
+    """Bit for bit: rows that share a product with it are not done in another order for it."""
+    gen = generator(96)
+    H, KH, D = 8, 2, 64
+    q, k, v = rnd(gen, dtype, n, H, D), rnd(gen, dtype, n, KH, D), rnd(gen, dtype, n, KH, D)
+    broken = q.clone()
+    broken[77, 1], broken[n - 1, 5, 3] = math.nan, math.nan
+    for (name, first, good), (_, _, out) in zip(every_form(q, k, v), every_form(broken, k, v)):
+        hit = torch.isnan(broken[first:]).any(-1)
+        assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], good[~hit]), name
