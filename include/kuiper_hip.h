@@ -162,6 +162,9 @@ int kh_scale_sum_f32(const float* value, const float* scale, float* out, int32_t
  * begin.  Rows are described by strides, in elements: [token][head][element], the elements of a head side by side.  A query
  * head h goes with key head h / (head_num / kv_head_num).
  *
+ * Rows that a call writes lie apart, their strides within one another in any order (a stride of zero over more than one row is
+ * refused).
+ *
  * Types: KH_DTYPE_BF16, KH_DTYPE_F32 (sums, softmax and angles in fp32 or more either way; attention in fp32 keeps fewer bits
  * of numbers below 2^-110).  Pointers are aligned to 16
  * bytes; head sizes and strides are multiples of 16 bytes; head_size and value_size are at most 256, a rotation has
@@ -193,7 +196,8 @@ int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scaling* scaling 
                   float* h_magnitude);
 
 /* The first rot_dim elements of every head are rotated by their token's position (any int32), the others pass; mode as in
- * kh_rope_f32.  q_out / k_out may be q / k, with the same strides (refused with others); they may not overlap them otherwise. */
+ * kh_rope_f32.  q_out / k_out may be q / k, with the same strides (refused with others); they may not overlap them, nor one
+ * another, otherwise. */
 typedef struct kh_rope_rows {
   int32_t dtype, mode, n_tokens, head_num, kv_head_num, head_size, rot_dim;
   float magnitude;
@@ -221,7 +225,7 @@ typedef struct kh_attn_rows {
   const int32_t* offsets;     /* [n_seqs + 1], ascending, at most n_tokens */
   const void* q;              /* [n_tokens][head_num][head_size] */
   int64_t q_token, q_head;
-  void* out;                  /* [n_tokens][head_num][value_size]; may not overlap q (refused where it is q) */
+  void* out;                  /* [n_tokens][head_num][value_size]; may not overlap q, keys or values (refused where it is one) */
   int64_t o_token, o_head;
 } kh_attn_rows;
 /* Whole prompts: the keys and values of a sequence are the rows of its own tokens. */

@@ -6,6 +6,7 @@
 // turn with an error of |p| 2^-54 turns (the table's own: f_i has 53 bits), where fp32 loses p f_i 2^-24 radians: 0.004 at
 // position 131072.  Its two highest bits, rounded, are the quadrant, and sine and cosine of what is left (at most an eighth of a
 // turn either way) are the Taylor polynomials, cut where the rest is below 2^-25.
+#include "kh_rows.h"
 #include "kh_tile.h"
 
 #include <math.h>
@@ -210,20 +211,21 @@ int go(const RopeArgs<T>& a, hipStream_t s) {
   return kh_launch_status();
 }
 
-// Elements of a row that is asked for by 16 bytes.
-bool whole(int64_t n, int esize) { return n % (16 / esize) == 0; }
-
 int check_rows(const kh_rope_rows* r, bool store) {
   if (!r || (r->dtype != KH_DTYPE_BF16 && r->dtype != KH_DTYPE_F32) || (r->mode != KH_ROPE_HALF && r->mode != KH_ROPE_INTERLEAVED) ||
       r->n_tokens < 0 || r->head_num <= 0 || r->kv_head_num <= 0 || r->head_num % r->kv_head_num || r->head_size <= 0 || r->rot_dim < 0 ||
       r->rot_dim % 2 || r->rot_dim > r->head_size || !(fabsf(r->magnitude) <= 3.4e38f))
     return KH_ERR_INVALID_ARG;
   const int e = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
-  if (!whole(r->head_size, e) || r->head_size > 256 || r->n_tokens >= 1 << 24) return KH_ERR_UNSUPPORTED;  // a grid has 2^32 threads
+  if (!rows_whole(r->head_size, e) || r->head_size > 256 || r->n_tokens >= 1 << 24) return KH_ERR_UNSUPPORTED;  // a grid has 2^32 threads
   if (r->n_tokens == 0) return KH_OK;
   if ((r->rot_dim && !r->turns) || !r->positions || !r->q || !r->k || !r->q_out || (!store && !r->k_out) || !kh_aligned16(r->q) || !kh_aligned16(r->k) ||
-      !kh_aligned16(r->q_out) || (!store && !kh_aligned16(r->k_out)) || !whole(r->q_token, e) || !whole(r->q_head, e) || !whole(r->k_token, e) ||
-      !whole(r->k_head, e) || !whole(r->qo_token, e) || !whole(r->qo_head, e) || (!store && (!whole(r->ko_token, e) || !whole(r->ko_head, e))))
+      !kh_aligned16(r->q_out) || (!store && !kh_aligned16(r->k_out)) || !rows_whole(r->q_token, e) || !rows_whole(r->q_head, e) || !rows_whole(r->k_token, e) ||
+      !rows_whole(r->k_head, e) || !rows_whole(r->qo_token, e) || !rows_whole(r->qo_head, e) || (!store && (!rows_whole(r->ko_token, e) || !rows_whole(r->ko_head, e))))
+    return KH_ERR_INVALID_ARG;
+  // a result has a place of its own
+  if ((!store && r->q_out == r->k_out) || !rows_apart({r->n_tokens, r->head_num}, {r->qo_token, r->qo_head}, r->head_size) ||
+      (!store && !rows_apart({r->n_tokens, r->kv_head_num}, {r->ko_token, r->ko_head}, r->head_size)))
     return KH_ERR_INVALID_ARG;
   // in place: a row is written where it was read
   auto moved = [&](int64_t token, int64_t head, int64_t o_token, int64_t o_head, int heads) {
@@ -339,11 +341,13 @@ extern "C" int kh_rope_store(const kh_rope_rows* r, const void* v, int64_t v_tok
   if (rc != KH_OK) return rc;
   const int e = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
   if (value_size <= 0) return KH_ERR_INVALID_ARG;
-  if (!khm::whole(value_size, e) || value_size > 256) return KH_ERR_UNSUPPORTED;
+  if (!khm::rows_whole(value_size, e) || value_size > 256) return KH_ERR_UNSUPPORTED;
   if (r->n_tokens == 0) return KH_OK;
   if (!v || !c || !slots || !c->k || !c->v || c->n_pages <= 0 || c->page_size <= 0 || !kh_aligned16(v) || !kh_aligned16(c->k) ||
-      !kh_aligned16(c->v) || !khm::whole(v_token, e) || !khm::whole(v_head, e) || !khm::whole(c->k_page, e) || !khm::whole(c->k_slot, e) ||
-      !khm::whole(c->k_head, e) || !khm::whole(c->v_page, e) || !khm::whole(c->v_slot, e) || !khm::whole(c->v_head, e))
+      !kh_aligned16(c->v) || !khm::rows_whole(v_token, e) || !khm::rows_whole(v_head, e) || !khm::rows_whole(c->k_page, e) || !khm::rows_whole(c->k_slot, e) ||
+      !khm::rows_whole(c->k_head, e) || !khm::rows_whole(c->v_page, e) || !khm::rows_whole(c->v_slot, e) || !khm::rows_whole(c->v_head, e) ||
+      c->k == c->v || !khm::rows_apart({c->n_pages, c->page_size, r->kv_head_num}, {c->k_page, c->k_slot, c->k_head}, r->head_size) ||
+      !khm::rows_apart({c->n_pages, c->page_size, r->kv_head_num}, {c->v_page, c->v_slot, c->v_head}, value_size))
     return KH_ERR_INVALID_ARG;
   return r->dtype == KH_DTYPE_BF16 ? khm::store<khm::bf16>(r, v, v_token, v_head, value_size, c, slots, (hipStream_t)stream)
                                    : khm::store<float>(r, v, v_token, v_head, value_size, c, slots, (hipStream_t)stream);

@@ -1,12 +1,11 @@
 // kh_seqattn.hip — attention of many sequences' tokens: checks and launches (kernels in kh_seqattn.h).
+#include "kh_rows.h"
 #include "kh_seqattn.h"
 
 #include <limits.h>
 
 namespace khm {
 namespace {
-
-bool whole(int64_t n, int esize) { return n % (16 / esize) == 0; }
 
 // Common checks; *todo = 0: nothing to do.
 int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
@@ -16,13 +15,14 @@ int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
       !(r->scale < INFINITY))
     return KH_ERR_INVALID_ARG;
   const int e = *esize = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
-  if (!whole(r->head_size, e) || !whole(r->value_size, e) || r->head_size > 256 || r->value_size > 256) return KH_ERR_UNSUPPORTED;
+  if (!rows_whole(r->head_size, e) || !rows_whole(r->value_size, e) || r->head_size > 256 || r->value_size > 256) return KH_ERR_UNSUPPORTED;
   // rows of a sequence are counted in 32 bits, and a grid has 2^32 threads
   if ((int64_t)r->n_tokens * r->head_num > INT_MAX / 2 || (int64_t)r->n_tokens * r->head_num / 128 + (int64_t)r->n_seqs * r->kv_head_num >= 1 << 24)
     return KH_ERR_UNSUPPORTED;
   if (r->n_tokens == 0 || r->n_seqs == 0) return KH_OK;
-  if (!r->offsets || !r->q || !r->out || r->q == r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !whole(r->q_token, e) || !whole(r->q_head, e) ||
-      !whole(r->o_token, e) || !whole(r->o_head, e))
+  if (!r->offsets || !r->q || !r->out || r->q == r->out || !kh_aligned16(r->q) || !kh_aligned16(r->out) || !rows_whole(r->q_token, e) || !rows_whole(r->q_head, e) ||
+      !rows_whole(r->o_token, e) || !rows_whole(r->o_head, e) ||
+      !rows_apart({r->n_tokens, r->head_num}, {r->o_token, r->o_head}, r->value_size))
     return KH_ERR_INVALID_ARG;
   *todo = 1;
   return KH_OK;
@@ -115,8 +115,8 @@ extern "C" int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_to
   int e, todo;
   const int rc = khm::check_rows(r, &e, &todo);
   if (rc != KH_OK || !todo) return rc;
-  if (!k || !v || !kh_aligned16(k) || !kh_aligned16(v) || !khm::whole(k_token, e) || !khm::whole(k_head, e) || !khm::whole(v_token, e) ||
-      !khm::whole(v_head, e))
+  if (!k || !v || k == r->out || v == r->out || !kh_aligned16(k) || !kh_aligned16(v) || !khm::rows_whole(k_token, e) || !khm::rows_whole(k_head, e) || !khm::rows_whole(v_token, e) ||
+      !khm::rows_whole(v_head, e))
     return KH_ERR_INVALID_ARG;
   khm::SeqRowsArgs ra{khm::args_of(r, e)};
   khm::SeqArgs& a = ra.s;
@@ -146,9 +146,9 @@ extern "C" int kh_attn_paged(const kh_attn_rows* r, const kh_page_cache* c, cons
   if (!c || c->n_pages <= 0 || c->page_size <= 0 || c->page_size > 1 << 20 || table_width <= 0 || table_stride < 0 || max_new < 0)
     return KH_ERR_INVALID_ARG;
   if (!todo) return KH_OK;
-  if (!c->k || !c->v || !pages || !lengths || !kh_aligned16(c->k) || !kh_aligned16(c->v) || !khm::whole(c->k_page, e) ||
-      !khm::whole(c->k_slot, e) || !khm::whole(c->k_head, e) || !khm::whole(c->v_page, e) || !khm::whole(c->v_slot, e) ||
-      !khm::whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
+  if (!c->k || !c->v || c->k == r->out || c->v == r->out || !pages || !lengths || !kh_aligned16(c->k) || !kh_aligned16(c->v) || !khm::rows_whole(c->k_page, e) ||
+      !khm::rows_whole(c->k_slot, e) || !khm::rows_whole(c->k_head, e) || !khm::rows_whole(c->v_page, e) || !khm::rows_whole(c->v_slot, e) ||
+      !khm::rows_whole(c->v_head, e) || !workspace || !kh_aligned16(workspace) ||
       workspace_bytes < kh_attn_paged_workspace_bytes(r->head_num, r->kv_head_num, r->value_size, r->n_tokens))
     return KH_ERR_INVALID_ARG;
   khm::SeqRowsArgs ra{khm::args_of(r, e), (int*)workspace, (float*)workspace + 2 * khm::SEQ_SHARES};

@@ -242,3 +242,28 @@ def test_pages_of_every_size_divide_exactly():
             for n in (q * d - 1, q * d, q * d + 1):
                 if 0 <= n < 2 ** 31:
                     assert ((n * magic) >> 32) >> (b - 1) == n // d, (d, n)
+
+
+def test_outputs_whose_rows_lie_in_one_another_are_refused(lib):
+    """An expanded tensor, or strides shorter than what lies within them: several workgroups would write one place, and a rotation in place
+    would turn a row that heads share once a head.  Of one row a stride says nothing."""
+    packed = lambda k=3 * P, v=4 * P, **kw: lib.kh_attn_packed(C.byref(attn_rows(**kw)), k, 128, 64, v, 128, 64, None)  # noqa: E731
+    paged = lambda c=cache(k=3 * P, v=4 * P), **kw: lib.kh_attn_paged(C.byref(attn_rows(**kw)), C.byref(c), P, 4, 4, P, 0, P, 1 << 40, None)  # noqa: E731
+    apart = dict(q_out=2 * P, k_out=3 * P)
+    tokens = lambda **kw: lib.kh_rope_tokens(C.byref(rope_rows(**{**apart, **kw})), None)  # noqa: E731
+    store = lambda c=cache(v=3 * P), **kw: lib.kh_rope_store(C.byref(rope_rows(**{**apart, **kw})), P, 128, 64, 64, C.byref(c), P, None)  # noqa: E731
+    for token, head in ((0, 64), (256, 0), (0, 0), (192, 64), (256, 56), (64, 64), (-192, 64), (64, 128)):
+        for call in (packed, paged):
+            assert call(o_token=token, o_head=head) == -1, (token, head)
+        for call in (tokens, store):
+            assert call(qo_token=token, qo_head=head) == -1, (token, head)
+    for token, head in ((0, 64), (128, 0), (64, 64)):
+        assert tokens(ko_token=token, ko_head=head) == -1, (token, head)
+        assert tokens(k_out=P, k_token=token, k_head=head, ko_token=token, ko_head=head) == -1, "in place"
+    for bad in (dict(k_page=0), dict(k_slot=0), dict(k_head=0), dict(v_page=1984), dict(v_slot=64), dict(v_head=8)):
+        assert store(c=cache(**{"v": 3 * P, **bad})) == -1, bad
+    # one place for two results, a result where keys or values are still to be read
+    assert tokens(k_out=2 * P) == -1
+    assert store(c=cache()) == -1  # k and v
+    assert packed(k=2 * P) == -1 and packed(v=2 * P) == -1
+    assert paged(c=cache(k=2 * P, v=4 * P)) == -1 and paged(c=cache(k=3 * P, v=2 * P)) == -1

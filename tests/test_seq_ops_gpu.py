@@ -818,3 +818,34 @@ def test_a_query_that_is_no_number_leaves_the_others_as_they_are(gpu, dtype, n):
     for (name, first, good), (_, _, out) in zip(every_form(q, k, v), every_form(broken, k, v)):
         hit = torch.isnan(broken[first:]).any(-1)
         assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], good[~hit]), name
+
+
+def test_outputs_of_any_layout_without_overlaps(gpu):
+    """Heads outside tokens, wider rows, one token with any stride, pages within slots: as contiguous ones; expanded tensors are refused."""
+    from kuiperllama_amd import _ffi, ops
+    gen = generator(97)
+    T, H, KH, D, pages, page = 20, 4, 2, 64, 5, 16
+    q, k, v = rnd(gen, BF16, T, H, D), rnd(gen, BF16, T, KH, D), rnd(gen, BF16, T, KH, D)
+    off, pos = offsets_of([T], gpu), torch.arange(T, dtype=torch.int32, device=gpu)
+    table = ops.rope_table(D, 1e4, gpu)
+    empty = lambda *s: torch.zeros(*s, dtype=BF16, device=gpu)  # noqa: E731
+    want = ops.attn_packed(q, k, v, off, empty(T, H, D))
+    for out in (empty(H, T, D).transpose(0, 1), empty(T, H, 2 * D)[..., D:], empty(T, 3, H, D)[:, 1]):
+        assert torch.equal(ops.attn_packed(q, k, v, off, out), want)
+    one = ops.attn_packed(q[:1], k[:1], v[:1], offsets_of([1], gpu), empty(1, H, D).as_strided((1, H, D), (0, D, 1)))
+    assert torch.equal(one, want[:1])
+    wants = ops.rope_tokens(q, k, pos, table, ops.ROPE_HALF, empty(T, H, D), empty(T, KH, D))
+    got = ops.rope_tokens(q, k, pos, table, ops.ROPE_HALF, empty(H, T, D).transpose(0, 1), empty(KH, T, D).transpose(0, 1))
+    assert torch.equal(got[0], wants[0]) and torch.equal(got[1], wants[1])
+    caches = []
+    for make in (lambda: empty(pages, page, KH, D), lambda: empty(page, KH, pages, D).permute(2, 0, 1, 3), lambda: empty(KH, pages, page, D).permute(1, 2, 0, 3)):
+        kc, vc = make(), make()
+        ops.rope_store(q, k, v, pos, table, ops.ROPE_HALF, kc, vc, pos, q_out=empty(T, H, D))
+        caches.append((kc, vc))
+    for kc, vc in caches[1:]:
+        assert torch.equal(kc, caches[0][0]) and torch.equal(vc, caches[0][1])
+    for bad in (lambda: ops.attn_packed(q, k, v, off, empty(T, 1, D).expand(T, H, D)), lambda: ops.attn_packed(q, k, v, off, empty(1, H, D).expand(T, H, D)),
+                lambda: ops.rope_tokens(q, k[:, :1].expand(T, KH, D), pos, table, ops.ROPE_HALF), lambda: ops.attn_packed(q, q, q, off, q),
+                lambda: ops.rope_store(q, k, v, pos, table, ops.ROPE_HALF, empty(pages, page, 1, D).expand(pages, page, KH, D), empty(pages, page, KH, D), pos)):
+        with pytest.raises(_ffi.KhError):
+            bad()
