@@ -306,6 +306,7 @@ extern "C" int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scalin
     lo = lo > 0 ? lo : 0;
     hi = hi < rot_dim - 1 ? hi : rot_dim - 1;
     *h_magnitude = (float)(c->magnitude > 0 ? c->magnitude : (c->factor > 1 ? 0.1 * log(c->factor) + 1.0 : 1.0));
+    if (!(*h_magnitude < INFINITY)) return KH_ERR_INVALID_ARG;
   }
   for (int i = 0; i < rot_dim / 2; ++i) {
     double f = pow(theta, -2.0 * i / rot_dim);
@@ -322,6 +323,7 @@ extern "C" int kh_rope_turns(int32_t rot_dim, double theta, const kh_rope_scalin
       f = f / c->factor * g + f * (1 - g);
     }
     double turn = f / two_pi;
+    if (!(turn < INFINITY)) return KH_ERR_INVALID_ARG;  // theta, factor or a border beyond what a frequency holds
     turn -= floor(turn);  // a frequency may be of more than a turn
     h_turns[i] = (uint64_t)ldexp(turn, 64);
   }

@@ -267,3 +267,16 @@ def test_outputs_whose_rows_lie_in_one_another_are_refused(lib):
     assert store(c=cache()) == -1  # k and v
     assert packed(k=2 * P) == -1 and packed(v=2 * P) == -1
     assert paged(c=cache(k=2 * P, v=4 * P)) == -1 and paged(c=cache(k=3 * P, v=2 * P)) == -1
+
+
+def test_turns_that_are_no_numbers_are_refused(lib):
+    """Frequencies and factors beyond what a number holds: there is no fraction of a turn to give."""
+    u, m = (C.c_uint64 * 128)(), C.c_float()
+    S = _ffi.RopeScaling
+    for theta, s in ((1e-299, S(kind=1, factor=1e-299)), (1e4, S(kind=1, factor=5e-324)), (1e4, S(kind=2, factor=5e-324, original=8192.0, low=1.0, high=4.0)),
+                     (1e4, S(kind=2, factor=8.0, original=math.inf, low=1.0, high=math.inf)),
+                     (1e4, S(kind=3, factor=5e-324, original=4096.0, fast=32.0, slow=1.0)),
+                     (1e4, S(kind=3, factor=8.0, original=4096.0, fast=32.0, slow=1.0, magnitude=math.inf)),
+                     (1e4, S(kind=3, factor=8.0, original=4096.0, fast=32.0, slow=1.0, magnitude=1e39))):
+        assert lib.kh_rope_turns(256, theta, C.byref(s), u, C.byref(m)) == -1, (theta, s.kind)
+    assert lib.kh_rope_turns(256, 1e-299, None, u, C.byref(m)) == 0  # the fastest pair: 1e296 radians a position, and a number
