@@ -849,3 +849,32 @@ def test_outputs_of_any_layout_without_overlaps(gpu):
                 lambda: ops.rope_store(q, k, v, pos, table, ops.ROPE_HALF, empty(pages, page, 1, D).expand(pages, page, KH, D), empty(pages, page, KH, D), pos)):
         with pytest.raises(_ffi.KhError):
             bad()
+
+
+# ---- tiles enough for the chip, sequences by the hundred -------------------------------------------------------------------
+MANY = [  # heads, kv_heads, key size, value size, new tokens, lengths, page, window
+    (32, 8, 128, 128, [2100], [2900], 16, 0), (32, 8, 128, 128, [1500, 650], [1500, 900], 24, 333),  # 525 tiles
+    (64, 64, 96, 96, [1100, 1], [1300, 500], 16, 0), (64, 64, 80, 80, [1100], [1200], 7, 100),  # 550
+    (64, 64, 256, 256, [600], [800], 16, 0), (40, 40, 192, 128, [840, 3], [900, 77], 1, 0),  # 300 and 280, of 256 columns
+    (8, 2, 96, 96, [100, 1, 40], [1000, 300, 40], 16, 0), (8, 2, 80, 88, [150], [700], 5, 90),  # a portion of 65 to 96 columns, in parts
+    (4, 2, 64, 64, [1] * 600, [1 + 37 * b % 419 for b in range(600)], 16, 0), (4, 1, 128, 128, [b % 3 for b in range(300)], [b % 3 + b for b in range(300)], 16, 50),
+    (2, 1, 64, 64, [1] * 500 + [60] + [1] * 550 + [40], [1 + b % 61 for b in range(500)] + [600] + [3] * 550 + [41], 16, 0)]  # more slots than are cut
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: str(c)[:60])
+def test_many_tiles_and_many_sequences(gpu, dtype, case):
+    from kuiperllama_amd import ops
+    H, KH, D, DV, new, lens, page, window = case
+    gen = generator(len(lens) + D)
+    kc, vc, table, ks, vs = paged(gen, dtype, KH, D, DV, lens, page)
+    T = sum(new)
+    q = rnd(gen, dtype, T + 1, H, D, scale=1.5)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    ws = ops.attn_paged_workspace(H, KH, DV, T + 1, gpu)
+    for max_new in (None, max(new)) if max(new) < 32 else (None,):
+        out = torch.full((T + 1, H, DV), 9.0, dtype=dtype, device=gpu)
+        ops.attn_paged(q, kc, vc, table, lengths, offsets_of(new, gpu), out, ws, window=window, max_new=max_new)
+        check_paged(q, out, lens, new, ks, vs, window, f"max_new {max_new}")
+        assert (out[T:] == 9.0).all()
+    assert not ws[:4096].any()
