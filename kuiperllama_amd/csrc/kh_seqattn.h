@@ -1186,10 +1186,11 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)kh_lds_addr(smem_raw));
   // ---- steps of every slot, slot i a thread's of number i mod 256
-  for (int i = threadIdx.x; i <= a.n_seqs && i < SEQ_TAB; i += 256) tab[i] = a.offsets[i];
+  static_assert(S::MOST <= SEQ_TAB, "a sequence has a slot at least, so that the table has room for all offsets");
+  for (int i = threadIdx.x; i < a.n_seqs; i += 256) tab[i] = a.offsets[i];
   __syncthreads();
   auto base_of = [&](int b) __attribute__((always_inline)) {
-    const int o = b < SEQ_TAB ? tab[b] : a.offsets[b];
+    const int o = tab[b];
     return (int)((int64_t)(o < 0 ? 0 : (o > a.n_tokens ? a.n_tokens : o)) * a.group / S::BM) + b;
   };
   constexpr int PER = S::MOST / 256;
