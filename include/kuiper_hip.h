@@ -235,7 +235,8 @@ int kh_attn_packed(const kh_attn_rows* r, const void* k, int64_t k_token, int64_
  * them.  pages: rows of page numbers, table_width of them a sequence, table_stride apart.  A page outside the cache or a
  * length behind the table makes rows that would need it NaN, and maybe others of that sequence; pages that no query of the
  * pass sees (behind the length, before the window) are not looked at.  max_new: the most new tokens that the caller
- * expects of any sequence (0: not known); it chooses between kernels and changes no result but by the order of sums.
+ * expects of any sequence (0: not known); it chooses between kernels and changes no result beyond its roundings.  Not known, a
+ * step of single tokens may take up to twice as long.
  * workspace = kh_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, ZEROED once before first use (the kernel leaves it
  * so where it counts); two calls, or two captured graphs, that may run at the same time need one each. */
 int64_t kh_attn_paged_workspace_bytes(int32_t head_num, int32_t kv_head_num, int32_t value_size, int32_t n_tokens);

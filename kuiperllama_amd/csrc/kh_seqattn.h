@@ -675,9 +675,9 @@ __device__ __forceinline__ void seq_tile_write(const SeqArgs& a, SeqTile& s, con
 }
 
 // Four waves of 32 rows each share the tiles of keys and values.  grid (slots * kv_heads): the key heads side by side, so that a
-// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.  8192 tokens of 32 heads over 8: 320 us at heads of
-// 64 (863 TFLOP/s), 585 at 128 (945), where the chip clocks down to 1.86 GHz and the matrix cores are busy 44 % of its cycles, the vector
-// unit (exponentials, maxima) 53.
+// key head's tiles stay with one XCD's L2 where their number is a multiple of eight.  8192 tokens of 32 heads over 8: 308 us at heads of
+// 64 (893 TFLOP/s; the chip clocks down to 1.82 GHz, the matrix cores are busy 43 % of its cycles, the vector unit with its exponentials and
+// maxima 67), 575 at 128 (956; 2.0 GHz, 45 and 40).
 template <class T, int DP, bool PAGED>
 __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 3 : (DP <= 128 ? 2 : 1)) void k_seq_tiles(const SeqArgs a) {
   typedef SeqTiles<T, DP> S;
@@ -697,8 +697,10 @@ __global__ __launch_bounds__(256, DP <= 64 && sizeof(T) == 2 ? 3 : (DP <= 128 ? 
 }
 
 // ---- few rows a sequence ---------------------------------------------------------------------------------------------------------
-// Sequences of up to 32 query rows (single tokens above all) read their keys once, whatever is done: HBM bounds them, so all keys
-// of all sequences are dealt evenly to the workgroups that fit on the chip at once.  A unit is a key head of a sequence; units lie one
+// Sequences of up to 32 query rows (single tokens above all) read their keys once, whatever is done: memory bounds them, so all keys
+// of all sequences are dealt evenly to the workgroups that fit on the chip at once.  One token over 131072 keys of 8 heads of 64
+// 61.5 us, 64 over 90 - 8106 keys of 8 heads of 128 115: 4.4 TB/s, not far from a copy's rate; requests alone, by the same instruction, have reached
+// 5.9 and, as read once, 7.1, and what lies between is not told apart.  A unit is a key head of a sequence; units lie one
 // behind the other, each a head and a number of steps of 128 keys, and workgroup i takes places [i W / N, (i + 1) W / N) of the W, the
 // end of one unit and the beginning of the next where they fall so.  What it finds of a unit that others have parts of goes to
 // the workspace, fp32 and with its m and l; the workgroup that is the last to bring a part adds them, in the order of the keys whoever
@@ -1359,7 +1361,9 @@ __device__ __forceinline__ void seq_tile_shares(const SeqRowsArgs& ra, int slots
 // Sequences of many rows and of few at once: half as many workgroups as the chip holds for the keys of the few between the first half
 // for parts of tiles and the rest of those, so that both kinds are there from the start.  Two portions of a prompt among 30 single
 // tokens, 32 heads of 64 over 4: 26 us (the portions alone 23, the single tokens alone 18), 34.5 with all for tiles ahead of as many
-// for the few.  At heads of 256 each kind fills the registers, and they are launches of their own.
+// for the few.  Either kind then has the other's registers, and the LDS of the larger: fp32 above 64 columns, where the rows' rings take 133 KB,
+// one workgroup a CU for the tiles too, which alone would be two.  At heads of 256 each kind fills the registers, and they are
+// launches of their own.
 template <class T, int DP>
 struct SeqMixed {
   static constexpr int LDS = SeqTiles<T, DP>::LDS_SHARES > SeqRows<T, DP>::LDS ? SeqTiles<T, DP>::LDS_SHARES : SeqRows<T, DP>::LDS;

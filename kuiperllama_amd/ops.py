@@ -271,6 +271,8 @@ def attn_paged(q, kcache, vcache, pages, lengths, offsets, out, workspace, scale
                max_new: Optional[int] = None):
     """Causal attention of the new tokens of each sequence, q [tokens, heads, size], sequence b the tokens offsets[b] .. offsets[b + 1] - 1,
     over the lengths[b] keys that the pages pages[b] (int32 [sequences, most pages]) of the cache hold of it, the new ones the
-    last of them.  window, scale: as attn_packed.  max_new: the most new tokens of a sequence, where the caller knows it (it
-    chooses the kernel).  workspace: attn_paged_workspace(...), not shared by calls that may run at the same time.  -> out"""
+    last of them.  window, scale: as attn_packed.  max_new: the most new tokens of a sequence, where the caller knows it: it
+    chooses the kernel, and without it a step of single tokens of more than 32 rows in all (tokens times heads / kv_heads) goes to the
+    one for portions of prompts, 4 - 8 % slower in bfloat16, up to twice as slow in float32.  workspace: attn_paged_workspace(...), not
+    shared by calls that may run at the same time.  -> out"""
     return _n.attn_paged(q, offsets, out, scale, window, kcache, vcache, pages, lengths, workspace, max_new or 0)
