@@ -430,9 +430,10 @@ __device__ __forceinline__ int seq_table(const SeqKv& kv, const int32_t* table, 
 // rows where that seems to have happened, and for those whose weights add up to nothing though they see a key (its place is theirs):
 // c times their scores has no room in a number, or all of these are minus infinity, and the row is NaN, as of the formula.
 template <class T, bool PAGED>
-__device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char* q, char* out, int place, int lane) {
+__device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char* q, char* out, int place, int lane_) {
   typedef typename Tile<T>::frag frag;
-  constexpr int E = Tile<T>::N, DEEP = 8;  // values requested together
+  constexpr int E = Tile<T>::N, DEEP = 8;  // keys whose values are requested together
+  const int lane = seq_fresh<true>(lane_);  // nothing of this in registers over the caller's loop
   const int lo = a.window > 0 && place >= a.window ? place - a.window + 1 : 0, cols = a.vchunks * E;
   auto score = [&](int key, int64_t& vo) __attribute__((always_inline)) {
     float s = -INFINITY;
@@ -468,18 +469,21 @@ __device__ __forceinline__ void seq_one(const SeqArgs& a, SeqKeys& x, const char
       const float p = weight(score(k0 + lane, vo)) * share;
       const int n = place - k0 < 63 ? place - k0 + 1 : 64;
       for (int j0 = 0; j0 < n; j0 += DEEP) {
-        float v[DEEP][4];
+        T v[DEEP][4];  // the last key and column again where there are no more: a load that nothing has to decide about waits for nothing
 #pragma unroll
         for (int j = 0; j < DEEP; ++j) {
-          const T* row = (const T*)(x.v + __shfl((long long)vo, j0 + j));
+          const T* row = (const T*)(x.v + __shfl((long long)vo, j0 + j < n ? j0 + j : n - 1));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[j][i] = j0 + j < n && lane + 64 * i < cols ? (float)row[lane + 64 * i] : 0.f;
+          for (int i = 0; i < 4; ++i)
+            if (64 * i < cols) v[j][i] = row[lane + 64 * i < cols ? lane + 64 * i : cols - 1];
         }
 #pragma unroll
         for (int j = 0; j < DEEP; ++j) {
+          if (j0 + j >= n) continue;
           const float w = __shfl(p, j0 + j);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, v[j][i], o[i]);
+          for (int i = 0; i < 4; ++i)
+            if (64 * i < cols) o[i] = __builtin_fmaf(w, (float)v[j][i], o[i]);
         }
       }
     }
