@@ -216,9 +216,9 @@ int kh_rope_store(const kh_rope_rows* r, const void* v, int64_t v_token, int64_t
                   const kh_page_cache* cache, const int32_t* slots, void* stream);
 
 /* Causal attention.  Query i of a sequence with n tokens here and `length` keys stands at place p = length - n + i and sees
- * the keys j with p - window < j <= p (window <= 0: all up to p); out = sum_j softmax_j(scale q . k_j) v_j, scale > 0.  A query
- * that sees no key gets zeros, one whose scores are all minus infinity NaN.  Rows behind the last sequence are left as they
- * were.  Keys that a query does not see do not reach it, whatever they hold. */
+ * the keys j with p - window < j <= p (window <= 0: all up to p); out = sum_j softmax_j(scale q . k_j) v_j, 0 < scale <= 2.3e38.
+ * A query that sees no key gets zeros, one whose scores are all minus infinity NaN.  Rows behind the last sequence are left as
+ * they were.  Keys that a query does not see do not reach it, whatever they hold. */
 typedef struct kh_attn_rows {
   int32_t dtype, n_tokens, n_seqs, head_num, kv_head_num, head_size, value_size, window;
   float scale;

@@ -7,12 +7,14 @@
 namespace khm {
 namespace {
 
+constexpr float LOG2E = 1.4426950408889634f;
+
 // Common checks; *todo = 0: nothing to do.
 int check_rows(const kh_attn_rows* r, int* esize, int* todo) {
   *todo = 0;
   if (!r || (r->dtype != KH_DTYPE_BF16 && r->dtype != KH_DTYPE_F32) || r->n_tokens < 0 || r->n_seqs < 0 || r->head_num <= 0 ||
       r->kv_head_num <= 0 || r->head_num % r->kv_head_num || r->head_size <= 0 || r->value_size <= 0 || !(r->scale > 0.f) ||
-      !(r->scale < INFINITY))
+      !(r->scale * LOG2E < INFINITY))
     return KH_ERR_INVALID_ARG;
   const int e = *esize = r->dtype == KH_DTYPE_BF16 ? 2 : 4;
   if (!rows_whole(r->head_size, e) || !rows_whole(r->value_size, e) || r->head_size > 256 || r->value_size > 256) return KH_ERR_UNSUPPORTED;
@@ -46,7 +48,7 @@ SeqArgs args_of(const kh_attn_rows* r, int e) {
   a.vchunks = r->value_size * e / 16;
   // places and lengths stay below 2^30 either way: a window of more holds everything, and a place less one of no more has room in 32 bits
   a.window = r->window > INT_MAX / 2 ? 0 : r->window;
-  a.c = r->scale * 1.4426950408889634f;
+  a.c = r->scale * LOG2E;
   return a;
 }
 

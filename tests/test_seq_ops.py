@@ -280,3 +280,11 @@ def test_turns_that_are_no_numbers_are_refused(lib):
                      (1e4, S(kind=3, factor=8.0, original=4096.0, fast=32.0, slow=1.0, magnitude=1e39))):
         assert lib.kh_rope_turns(256, theta, C.byref(s), u, C.byref(m)) == -1, (theta, s.kind)
     assert lib.kh_rope_turns(256, 1e-299, None, u, C.byref(m)) == 0  # the fastest pair: 1e296 radians a position, and a number
+
+
+def test_scales_that_have_no_room_in_base_two_are_refused(lib):
+    """Exponentials run in base two: scale log2 e has to be a number too."""
+    for scale in (2.37e38, 3.4e38):
+        r = C.byref(attn_rows(scale=scale))
+        assert lib.kh_attn_packed(r, 3 * P, 128, 64, 4 * P, 128, 64, None) == -1, scale
+        assert lib.kh_attn_paged(r, C.byref(cache(k=3 * P, v=4 * P)), P, 4, 4, P, 0, P, 1 << 40, None) == -1, scale
